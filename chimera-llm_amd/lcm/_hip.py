@@ -16,6 +16,8 @@ LIB_PATH = os.environ.get("LCMHIP_LIB") or os.path.join(_HERE, "liblcm_hip.so")
 
 F32, BF16 = 0, 1
 NORM_LAYERNORM, NORM_RMS, NORM_FP32, NORM_UNIT = 0, 1, 2, 3
+NORM_NONE = -1                                   # HeadNorm only
+ROTARY = {"pairs": 0, "halves": 1}               # LCMHIP_ROTARY_*
 FFN_RELU, FFN_SWIGLU = 0, 1
 # LCMHIP_ACT_*: inner activation of the two-matrix FFN, by the reference's name (lcm/nn/initialization.py:121-151)
 ACT = {"relu": 0, "tanh": 1, "elu": 2, "leaky_relu": 3, "selu": 4, "gelu": 5, "silu": 6, "softsign": 7, "sigmoid": 8,
@@ -25,7 +27,7 @@ ORDER = {"pre": 0, "post": 1, "normformer": 2}   # LCMHIP_ORDER_*
 PRED = {"sample": 0, "epsilon": 1, "v_prediction": 2}
 EPI_STORE, EPI_STORE_F32, EPI_RELU, EPI_SWIGLU, EPI_RESID = 0, 1, 2, 3, 4
 STATIC_SCRATCH_BYTES = 16 << 20      # LCMHIP_STATIC_SCRATCH_BYTES of include/lcmhip.h
-ABI_VERSION = 401                    # LCMHIP_ABI_VERSION of include/lcmhip.h: the layouts and signatures bound below
+ABI_VERSION = 402                    # LCMHIP_ABI_VERSION of include/lcmhip.h: the layouts and signatures bound below
 # LCMHIP_SESSION_* flags of lcmhip_session_workspace_bytes / lcmhip_session_create
 SESSION_KEEP_CONTEXT, SESSION_SEPARATE_QKV, SESSION_SEPARATE_ROPE, SESSION_NO_GRAPH = 1, 2, 4, 8
 
@@ -40,6 +42,8 @@ EXPORTS = [
     "lcmhip_normalize", "lcmhip_denormalize", "lcmhip_rfft_pack", "lcmhip_norm_modulate", "lcmhip_gemm", "lcmhip_static_init", "lcmhip_gemm_static", "lcmhip_gemm_partial",
     "lcmhip_residual_norm",
     "lcmhip_ddim_cfg_step", "lcmhip_attention", "lcmhip_finalize_step", "lcmhip_stream_copy",
+    "lcmhip_head_norm_rope", "lcmhip_paged_append", "lcmhip_paged_attention_workspace", "lcmhip_paged_attention",
+    "lcmhip_shared_prefix_attention_workspace", "lcmhip_shared_prefix_attention",
 ]
 
 
@@ -68,6 +72,31 @@ class DenoiseParams(C.Structure):
 class ProfileRow(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("launches", C.c_int64), ("total_ms", C.c_double),
                 ("bytes", C.c_double), ("flops", C.c_double)]
+
+
+class KVPages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_int64), ("page_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("q_starts", C.c_void_p), ("n_seqs", C.c_int32),
+                ("max_pages", C.c_int32), ("max_q", C.c_int32), ("max_keys", C.c_int32)]
+
+
+class SharedPrefix(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("lens", C.c_void_p), ("group_starts", C.c_void_p), ("n_groups", C.c_int32),
+                ("max_pages", C.c_int32), ("max_keys", C.c_int32)]
+
+
+class HeadNorm(C.Structure):
+    _fields_ = [("q_weight", C.c_void_p), ("q_bias", C.c_void_p), ("k_weight", C.c_void_p), ("k_bias", C.c_void_p),
+                ("kind", C.c_int32), ("eps", C.c_float)]
+
+
+class Rotary(C.Structure):
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("n_positions", C.c_int32), ("rotary_dim", C.c_int32),
+                ("style", C.c_int32)]
 
 
 def _load() -> C.CDLL:
@@ -118,6 +147,17 @@ def _load() -> C.CDLL:
         "lcmhip_attention": [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp],
         "lcmhip_stream_copy": [vp, vp, i64, i32, vp],
         "lcmhip_finalize_step": [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp],
+        "lcmhip_head_norm_rope": [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, i64, i32, i32, i32,
+                                  C.POINTER(HeadNorm), C.POINTER(Rotary), vp, i32, vp],
+        "lcmhip_paged_append": [C.POINTER(KVPages), C.POINTER(PagedBatch), vp, i64, i64, vp, i64, i64, vp, i64, i64, vp,
+                                i64, i32, C.POINTER(HeadNorm), C.POINTER(Rotary), vp, vp],
+        "lcmhip_paged_attention_workspace": [C.POINTER(KVPages), C.POINTER(PagedBatch), i64, i32, C.POINTER(C.c_size_t)],
+        "lcmhip_paged_attention": [C.POINTER(KVPages), C.POINTER(PagedBatch), vp, i64, i64, vp, i64, i32, f32, i32, vp,
+                                   C.c_size_t, vp],
+        "lcmhip_shared_prefix_attention_workspace": [C.POINTER(KVPages), C.POINTER(PagedBatch), C.POINTER(SharedPrefix),
+                                                     i64, i32, C.POINTER(C.c_size_t)],
+        "lcmhip_shared_prefix_attention": [C.POINTER(KVPages), C.POINTER(PagedBatch), C.POINTER(SharedPrefix), vp, i64,
+                                           i64, vp, i64, i32, f32, i32, vp, C.c_size_t, vp],
     }
     for name, argtypes in sig.items():
         fn = getattr(lib, name)

@@ -33,13 +33,14 @@ extern "C" {
 #endif
 
 /* Version of this ABI (struct layouts and signatures).  lcmhip_version() returns the value the library was built
- * with; a caller built against another value must not bind.  400 -> 401: lcmhip_base_forward with normalized != 0
+ * with; a caller built against another value must not bind.  401 -> 402: the paged cache entry points added
+ * (lcmhip_head_norm_rope .. lcmhip_shared_prefix_attention; no earlier layout or signature changed).  400 -> 401: lcmhip_base_forward with normalized != 0
  * returns its predictions in the normalizer's space (it applied the inverse normalizer before).  300 -> 400: lcmhip_tower_desc.norm_order,
  * no_final_norm and scale_residual, LCMHIP_POS_SINE, LCMHIP_ACT_PRELU, lcmhip_model_desc.postnet_activation,
  * lcmhip_rfft_pack; 200 -> 300: lcmhip_session_workspace_bytes and
  * lcmhip_session_create take `flags`, lcmhip_static_init added, lcmhip_tower_desc.ffn_activation; 100 -> 200: lcmhip_tower_desc.qk_layernorm,
  * thresholding fields of lcmhip_denoise_params, variance_noise of lcmhip_ddim_cfg_step. */
-#define LCMHIP_ABI_VERSION 401
+#define LCMHIP_ABI_VERSION 402
 
 #define LCMHIP_OK 0
 #define LCMHIP_ERR_INVALID (-1)     /* bad argument / shape the kernels do not support */
@@ -402,6 +403,110 @@ int lcmhip_finalize_step(const float* new_emb, void* seqs, int32_t seqs_dtype, c
 int lcmhip_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* slot_map,
                      void* out, int32_t n_docs, int32_t s, int32_t n_heads, int32_t cap,
                      int32_t base_keys, int32_t causal, int32_t dtype, void* stream);
+
+/* ---- paged key/value cache ------------------------------------------------------------------
+ * No counterpart in the reference: its cache is one growing tensor per document (lcm/nn/incremental_state.py:14-43).
+ * Here the keys and values of a layer live in a pool of pages of `page_size` positions, a page belongs to any sequence
+ * whose table names it, and a batch is a ragged list of sequences.
+ *
+ * All index arrays are int32 DEVICE arrays that the kernels read when they run (so a captured graph may be replayed on new
+ * contents); the host numbers of the structs are bounds.  What the arrays say is never trusted with an address:
+ *  - a page id outside [0, n_pages) names a page that is not there: nothing is stored to it and its keys are left out;
+ *  - sequence lengths are cut to [0, min(max_keys, max_pages * page_size)], row ranges to [0, rows];
+ *  - rows that belong to no sequence (before q_starts[0], from q_starts[n_seqs] on) are neither read nor written.
+ * Row pointers are 16-byte aligned and their strides (in elements) a multiple of 16 bytes; the last dimension is dense.
+ * head_dim is 64 or 128, page_size a power of two >= 16, n_heads a multiple of n_kv_heads (query head h reads key head
+ * h / (n_heads / n_kv_heads)).  Outputs must not overlap inputs unless a comment says so. */
+enum { LCMHIP_NORM_NONE = -1 };                              /* lcmhip_head_norm only */
+enum { LCMHIP_ROTARY_PAIRS = 0, LCMHIP_ROTARY_HALVES = 1 };  /* pairs (2i, 2i + 1), or (i, i + rotary_dim / 2) */
+
+/* The page pool of one layer: k, v (n_pages, n_kv_heads, page_size, head_dim), contiguous. */
+typedef struct {
+    void* k;
+    void* v;
+    int64_t n_pages;
+    int32_t page_size, n_kv_heads, head_dim, dtype;
+} lcmhip_kv_pages;
+
+/* A ragged batch.  Sequence b owns rows [q_starts[b], q_starts[b + 1]) of the row tensors -- its newest positions, up to and
+ * including position seq_lens[b] - 1 -- and its position c lies in page page_table[b][c / page_size]. */
+typedef struct {
+    const int32_t* page_table; /* (n_seqs, max_pages) */
+    const int32_t* seq_lens;   /* (n_seqs) positions in the cache, the rows of this call included */
+    const int32_t* q_starts;   /* (n_seqs + 1) or NULL: one row for every sequence */
+    int32_t n_seqs, max_pages;
+    int32_t max_q;             /* the most rows of one sequence; chooses the kernel, a wrong value costs time only */
+    int32_t max_keys;          /* upper bound of seq_lens, <= max_pages * page_size */
+} lcmhip_paged_batch;
+
+/* Common beginnings: the sequences [group_starts[g], group_starts[g + 1]) continue the lens[g] positions of the pages
+ * page_table[g]; seq_lens and page_table of the batch then count a sequence's own positions only. */
+typedef struct {
+    const int32_t* page_table;   /* (n_groups, max_pages) */
+    const int32_t* lens;         /* (n_groups) */
+    const int32_t* group_starts; /* (n_groups + 1) sequence indices, not falling */
+    int32_t n_groups, max_pages;
+    int32_t max_keys;            /* upper bound of lens, <= max_pages * page_size */
+} lcmhip_shared_prefix;
+
+/* Norm over every head (weights and biases (head_dim,) in the operand dtype, one vector for all heads; biases for
+ * LCMHIP_NORM_LAYERNORM only and optional; none of them for LCMHIP_NORM_UNIT / LCMHIP_NORM_NONE). */
+typedef struct {
+    const void* q_weight;
+    const void* q_bias;
+    const void* k_weight;
+    const void* k_bias;
+    int32_t kind; /* LCMHIP_NORM_* or LCMHIP_NORM_NONE */
+    float eps;
+} lcmhip_head_norm;
+
+/* Rotation of the first rotary_dim dimensions (a multiple of 16 up to head_dim) of a head at position p by the angles whose
+ * cosines and sines are row p of cos / sin (n_positions, rotary_dim / 2) fp32. */
+typedef struct {
+    const float* cos;
+    const float* sin;
+    int32_t n_positions, rotary_dim;
+    int32_t style; /* LCMHIP_ROTARY_* */
+} lcmhip_rotary;
+
+/* Norm of every query and key head and the rotation behind it in one pass: y = rotate(norm(x)), fp32 inside, rounded once.
+ * q, q_out (rows, n_heads, head_dim), k, k_out (rows, n_kv_heads, head_dim) with row / head strides; either pair may be NULL.
+ * norm, rotary: NULL for none.  positions (rows) int32, required with rotary: rows of a negative position are skipped (q_out,
+ * k_out keep what they hold), a position >= n_positions gives NaN.  q_out may be q and k_out k (same strides). */
+int lcmhip_head_norm_rope(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                          void* q_out, int64_t q_out_row, int64_t q_out_head, void* k_out, int64_t k_out_row, int64_t k_out_head,
+                          int64_t rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const lcmhip_head_norm* norm,
+                          const lcmhip_rotary* rotary, const int32_t* positions, int32_t dtype, void* stream);
+
+/* Stores the batch's rows of k (normed and rotated as above) and v into the pages of their sequences; q (NULL: none) goes
+ * through the same norm and rotation into q_out, contiguous (rows, n_heads, head_dim), in the same pass.  Row t of sequence b has
+ * cache position c = seq_lens[b] - (q_starts[b + 1] - t); it is rotated by positions[t], or by c when positions is NULL.  Rows
+ * with c < 0, c beyond the table or a negative position are skipped.  Two sequences that name the same page write it both.
+ * rows: the rows that q, k and v hold. */
+int lcmhip_paged_append(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, const void* k, int64_t k_row, int64_t k_head,
+                        const void* v, int64_t v_row, int64_t v_head, const void* q, int64_t q_row, int64_t q_head, void* q_out,
+                        int64_t rows, int32_t n_heads, const lcmhip_head_norm* norm, const lcmhip_rotary* rotary,
+                        const int32_t* positions, void* stream);
+
+/* softmax(scale q K^T) V over the pages: with causal != 0 row t of sequence b sees the positions [0, seq_lens[b] -
+ * (q_starts[b + 1] - t) + 1), otherwise all seq_lens[b].  A row that sees no key gives zeros.  q (rows, n_heads, head_dim)
+ * strided, out the same contiguous; scale > 0.  Softmax statistics and sums are fp32.  `workspace` (device, 256-byte aligned) of at
+ * least lcmhip_paged_attention_workspace bytes holds partial results while the call runs; nothing in it has to be zero and
+ * nothing is kept in it between calls, but calls that may overlap must not share one.  bytes == 0: NULL will do. */
+int lcmhip_paged_attention_workspace(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, int64_t rows, int32_t n_heads,
+                                     size_t* bytes);
+int lcmhip_paged_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, const void* q, int64_t q_row, int64_t q_head,
+                           void* out, int64_t rows, int32_t n_heads, float scale, int32_t causal, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* lcmhip_paged_attention for sequences with common beginnings: every row sees all positions of its group's prefix and then its
+ * sequence's own ones (causal as above).  The prefix is read once for all rows of a group, and the two parts are joined by their
+ * softmax statistics.  Sequences in no group have no prefix. */
+int lcmhip_shared_prefix_attention_workspace(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch,
+                                             const lcmhip_shared_prefix* prefix, int64_t rows, int32_t n_heads, size_t* bytes);
+int lcmhip_shared_prefix_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, const lcmhip_shared_prefix* prefix,
+                                   const void* q, int64_t q_row, int64_t q_head, void* out, int64_t rows, int32_t n_heads, float scale,
+                                   int32_t causal, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
