@@ -1,100 +1,475 @@
 // Attention of a ragged batch over the pages of its sequences, with or without prefixes that groups of sequences share.
 //
-// One wave for each (row, query head); lane = (key slot ks = lane / 4, dim group dg = lane % 4) walks the keys ks, ks + 16, ..
-// with an online softmax (running maximum, sum and D / 4 accumulators a lane); the 16 slots are merged with shuffles at the
-// end.  Sixteen keys of one step lie in one page, whose id is read once for the step.
+//     o = sum_i exp(scale (x_i - m)) v_i / sum_i exp(scale (x_i - m)),   x_i = q . k_i,   m = max_i x_i
+//
+// in one pass over the keys with a running m, l = sum exp and o; two parts (m, l, o) of a row join as
+//     m = max(m1, m2),   l = l1 w1 + l2 w2,   o = o1 w1 + o2 w2,   w = exp(scale (m_i - m)).
+// The long axis is the keys': a sequence's keys are cut into parts that different workgroups walk, and k_paged_join joins
+// them.  A prefix that sequences share is one more list of parts, whose rows are all rows of the group.
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
 #include "paged.h"
 
 namespace lcmhip {
+
+using bf16x8_t = __attribute__((ext_vector_type(8))) __bf16;
+using u32x4_t = __attribute__((ext_vector_type(4))) uint32_t;
+using u32x2_t = __attribute__((ext_vector_type(2))) uint32_t;
+using f32x4_t = __attribute__((ext_vector_type(4))) float;
+
+// Lists of keys that rows attend to: a sequence's own positions, or the prefix of a group of sequences.
+struct KeyLists {
+    PageTable table;
+    const int32_t* lens;
+    const int32_t* group_starts;     // null: list i belongs to sequence i
+    int n, max_keys;
+    int causal;                      // row r of the list sees keys [0, len - rows + r + 1)
+    int splits, part0;               // parts of a list, and the number of the first
+};
 
 struct PagedArgs {
     const void* q; int64_t q_row, q_head;
     void* out;
     const void *kp, *vp;
-    PageTable table, prefix_table;
-    const int32_t *seq_lens, *q_starts, *prefix_lens, *group_starts;
-    int n_seqs, n_groups, max_keys, prefix_max_keys;
-    int64_t rows;
-    int hq, hk, causal;
+    const int32_t* q_starts;
+    int n_seqs, rows, hq, hk;
     float scale_log2;          // scale * log2(e).  It multiplies differences of dot products only: a product that fits fp32
                                // may leave it when multiplied by log2(e), and far from zero its rounding is no small number
+    float* part_o;             // [part][row][head][D], not divided by l; null: a single part, finished in place
+    float2* part_ml;           // [part][row][head] (m, l)
 };
 
+// Rows and keys of list i.
+__device__ __forceinline__ void list_extent(const PagedArgs& a, const KeyLists& ls, int i, int& r0, int& r1, int& keys) {
+    int s0 = i, s1 = i + 1;
+    if (ls.group_starts) {
+        s0 = min(max(ls.group_starts[i], 0), a.n_seqs);
+        s1 = min(max(ls.group_starts[i + 1], s0), a.n_seqs);
+    }
+    r0 = a.q_starts ? a.q_starts[s0] : s0;
+    r1 = a.q_starts ? a.q_starts[s1] : s1;
+    r0 = min(max(r0, 0), a.rows);
+    r1 = min(max(r1, r0), a.rows);
+    keys = max(0, min(ls.lens[i], ls.max_keys));
+}
+
+// Part `split` of `keys` keys: at most `splits` equal parts, multiples of 32 keys, of no fewer than kMinPart.
+constexpr int kMinPart = 256;
+__device__ __forceinline__ void part_range(int keys, int splits, int split, int& k0, int& k1) {
+    const int n = max(1, min(splits, (keys + kMinPart - 1) / kMinPart));
+    const int len = ((keys + n - 1) / n + 31) & ~31;
+    k0 = min(keys, split * len);
+    k1 = min(keys, k0 + len);
+}
+
+// ---- a tile of 16 rows against groups of keys, by one wave ------------------------------------------------------------------
+// Both products run on 16 x 16 matrix instructions with the keys (dims) as rows and the query rows as columns, so that a lane
+// keeps one query row (lane % 16) throughout and softmax statistics need no exchange but over the four quads (lane / 16):
+//     S^T[key][row] = K Q^T        lane holds keys 4 quad .. 4 quad + 3 of every 16
+//     O^T[dim][row] += V^T P^T      the lane's own probabilities are its P^T operand
+// The order of the inner index is free as long as both operands agree: key slots are numbered so that the operand P^T is
+// what the lane holds, and dim rows so that the operand V^T is what 16-byte loads of value rows bring (below).
+// No operand passes through LDS, and consecutive lanes read consecutive bytes.
+// Mask of the bf16 halves of a word that are NaN or infinite.
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+    return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
 template <typename T, int D>
-__global__ __launch_bounds__(64) void k_paged_rows(PagedArgs a) {
-    constexpr int P = D / 32;                       // 8-value pieces of a lane
-    const int64_t row = blockIdx.x / a.hq;
-    const int head = blockIdx.x % a.hq, hk = head / (a.hq / a.hk);
-    const int lane = threadIdx.x, ks = lane >> 2, dg = lane & 3;
-    const int seq = a.q_starts ? wave_count_le(a.q_starts + 1, a.n_seqs, row) : (int)row;
-    if (seq >= a.n_seqs) return;
-    int64_t r0, r1;
-    seq_rows(a.q_starts, seq, a.rows, r0, r1);
-    if (row < r0) return;
-    const int len = max(0, min(a.seq_lens[seq], a.max_keys));
-    const int keys = (int)max((int64_t)0, a.causal ? len - (r1 - row) + 1 : (int64_t)len);
-    int group = a.n_groups, prefix = 0;
-    if (a.n_groups > 0) {
-        group = wave_count_le(a.group_starts + 1, a.n_groups, seq);
-        if (group < a.n_groups && a.group_starts[group] <= seq) prefix = max(0, min(a.prefix_lens[group], a.prefix_max_keys));
+struct Tile16;
+
+template <int D>
+struct Tile16<bf16_t, D> {
+    static constexpr int kKeys = 32;                       // two 16-key halves, each in one page
+    static constexpr int kHalves = 2;
+    static constexpr int kO = D / 16;                      // accumulators; o[c][r] is dim kO * (4 quad + r) + c
+    using vpiece_t = typename std::conditional<D == 128, u32x4_t, u32x2_t>::type;   // kO consecutive dims of a value row
+    bf16x8_t q[D / 32], k[2][D / 32];
+    vpiece_t v[2][4];                                      // value row 4 quad + e of half h, dims kO * (lane % 16) ..
+
+    __device__ __forceinline__ void load_q(const bf16_t* row, bool live, int lane) {
+#pragma unroll
+        for (int st = 0; st < D / 32; ++st) {
+            u32x4_t x = {0, 0, 0, 0};
+            if (live) x = *reinterpret_cast<const u32x4_t*>(row + 32 * st + 8 * (lane >> 4));
+            q[st] = __builtin_bit_cast(bf16x8_t, x);
+        }
     }
-    const int col = dg * 8;
-    float qv[P][8];
+    __device__ __forceinline__ void load_k(int h, const bf16_t* base, int lane) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-        load8<T>(reinterpret_cast<const T*>(a.q) + row * a.q_row + head * a.q_head + col + 32 * i, qv[i]);
+        for (int st = 0; st < D / 32; ++st)
+            k[h][st] = *reinterpret_cast<const bf16x8_t*>(base + (lane & 15) * D + 32 * st + 8 * (lane >> 4));
     }
-    float m = -INFINITY, l = 0.f, acc[P][8] = {};
-    bool seen = false;
-    auto walk = [&](const PageTable& table, int which, int count) {
-        for (int k0 = 0; k0 < count; k0 += 16) {
-            const int page = table.page(which, k0);
-            if (page < 0) continue;
-            const int key = k0 + ks;
-            if (key >= count) continue;             // the 4 lanes of a slot agree
-            const size_t at = ((((size_t)page * a.hk + hk) << table.page_shift) + (key & ((1 << table.page_shift) - 1))) * D + col;
-            float s = 0.f, vv[P][8];
+    __device__ __forceinline__ void load_v(int h, const bf16_t* base, int lane) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                float kv[8];
-                load8<T>(reinterpret_cast<const T*>(a.kp) + at + 32 * i, kv);
-                load8<T>(reinterpret_cast<const T*>(a.vp) + at + 32 * i, vv[i]);
+        for (int e = 0; e < 4; ++e)
+            v[h][e] = *reinterpret_cast<const vpiece_t*>(base + (4 * (lane >> 4) + e) * D + kO * (lane & 15));
+    }
+    __device__ __forceinline__ void scores(float (&s)[8]) const {
 #pragma unroll
-                for (int t = 0; t < 8; ++t) s += kv[t] * qv[i][t];
+        for (int h = 0; h < 2; ++h) {
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < D / 32; ++st) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[h][st], q[st], acc, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * h + e] = acc[e];
+        }
+    }
+    __device__ __forceinline__ void clear_v(int h, int e) { v[h][e] = vpiece_t{}; }
+    __device__ __forceinline__ bool v_not_finite(int h, int e) const {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) bad |= not_finite(v[h][e][w]);
+        return bad != 0;
+    }
+    // V^T operand c: dim kO * (lane % 16) + c of the lane's 8 value rows, picked out of the pieces that hold kO dims of one row
+    __device__ __forceinline__ bf16x8_t v_operand(int c) const {
+        const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
+        u32x4_t x;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) x[2 * h + p] = __builtin_amdgcn_perm(v[h][2 * p + 1][c / 2], v[h][2 * p][c / 2], sel);
+        return __builtin_bit_cast(bf16x8_t, x);
+    }
+    // Probabilities are rounded to bf16 for the second product (relative 2^-8 each, like the values they weigh); their sum
+    // is taken before, in fp32.
+    __device__ __forceinline__ void weigh(const float (&p)[8], f32x4_t (&o)[kO]) const {
+        bf16x8_t pf;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pf[e] = (__bf16)p[e];
+#pragma unroll
+        for (int c = 0; c < kO; ++c) o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v_operand(c), pf, o[c], 0, 0, 0);
+    }
+    // The values of key i that are not finite alone, into the rows (lanes) that see it.
+    __device__ __forceinline__ void weigh_not_finite(const float (&p)[8], f32x4_t (&o)[kO], int i, bool visible, int lane) const {
+        bf16x8_t pf;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pf[e] = (__bf16)p[e];
+        const uint32_t mask = (lane >> 4) == ((i & 15) >> 2) ? ((i & 1) ? 0xffff0000u : 0x0000ffffu) : 0u;
+        const int word = 2 * (i >> 4) + ((i & 3) >> 1);
+#pragma unroll
+        for (int c = 0; c < kO; ++c) {
+            u32x4_t x = __builtin_bit_cast(u32x4_t, v_operand(c));
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x[w] = w == word ? x[w] & not_finite(x[w]) & mask : 0u;
+            const f32x4_t y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), pf, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[c][r] += visible ? y[r] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void clear_not_finite() {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int w = 0; w < D / 32; ++w) v[h][e][w] &= ~not_finite(v[h][e][w]);
+    }
+    __device__ static __forceinline__ int dim(int c, int r, int lane) { return kO * (4 * (lane >> 4) + r) + c; }
+};
+
+template <int D>
+struct Tile16<float, D> {
+    static constexpr int kKeys = 16;
+    static constexpr int kHalves = 1;
+    static constexpr int kO = D / 16;                      // o[4 u + c][r] is dim 64 u + 4 (4 quad + r) + c
+    f32x4_t q[D / 16], k[1][D / 16];                       // dims 16 i + 4 quad .. + 3
+    f32x4_t v[1][4][D / 64];                               // value row 4 quad + e, dims 64 u + 4 (lane % 16) .. + 3
+
+    __device__ __forceinline__ void load_q(const float* row, bool live, int lane) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            q[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (live) q[i] = *reinterpret_cast<const f32x4_t*>(row + 16 * i + 4 * (lane >> 4));
+        }
+    }
+    __device__ __forceinline__ void load_k(int, const float* base, int lane) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) k[0][i] = *reinterpret_cast<const f32x4_t*>(base + (lane & 15) * D + 16 * i + 4 * (lane >> 4));
+    }
+    __device__ __forceinline__ void load_v(int, const float* base, int lane) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int u = 0; u < D / 64; ++u)
+                v[0][e][u] = *reinterpret_cast<const f32x4_t*>(base + (4 * (lane >> 4) + e) * D + 64 * u + 4 * (lane & 15));
+    }
+    __device__ __forceinline__ void scores(float (&s)[4]) const {
+        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0][i][e], q[i][e], acc, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = acc[e];
+    }
+    __device__ __forceinline__ void clear_v(int, int e) {
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) v[0][e][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ bool v_not_finite(int, int e) const {
+        bool bad = false;
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) bad |= not_finite(v[0][e][u][c]);
+        return bad;
+    }
+    __device__ __forceinline__ void weigh(const float (&p)[4], f32x4_t (&o)[kO]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int u = 0; u < D / 64; ++u)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[4 * u + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0][e][u][c], p[e], o[4 * u + c], 0, 0, 0);
+    }
+    __device__ __forceinline__ void weigh_not_finite(const float (&p)[4], f32x4_t (&o)[kO], int i, bool visible, int lane) const {
+        const bool mine = (lane >> 4) == (i >> 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e != (i & 3)) continue;
+#pragma unroll
+            for (int u = 0; u < D / 64; ++u)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float x = v[0][e][u][c];
+                    const f32x4_t y = __builtin_amdgcn_mfma_f32_16x16x4f32(mine && not_finite(x) ? x : 0.f, p[e], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[4 * u + c][r] += visible ? y[r] : 0.f;
+                }
+        }
+    }
+    __device__ __forceinline__ void clear_not_finite() {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int u = 0; u < D / 64; ++u)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[0][e][u][c] = not_finite(v[0][e][u][c]) ? 0.f : v[0][e][u][c];
+    }
+    __device__ static __forceinline__ int dim(int c, int r, int lane) { return 64 * (c >> 2) + 4 * (4 * (lane >> 4) + r) + (c & 3); }
+};
+
+// Few rows for each list of keys: a tile of 16 (row, head of the group) pairs of one key head against one part of a list, four
+// waves that take the part's groups of keys in turn and join their results in LDS.  Bound by the bytes of the keys and values.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void k_paged_few(PagedArgs a, KeyLists ls, int row_tiles) {
+    using Tile = Tile16<T, D>;
+    constexpr int NP = 4 * Tile::kHalves, OROW = D + 4;
+    __shared__ float red_o[4][16][OROW];
+    __shared__ float2 red_ml[4][16];
+    const int lane = threadIdx.x & 63, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int bid = blockIdx.x;
+    const int hk = bid % a.hk;
+    bid /= a.hk;
+    const int split = bid % ls.splits;
+    bid /= ls.splits;
+    const int list = bid % ls.n, tile0 = bid / ls.n;
+    const int G = a.hq / a.hk;
+    int r0, r1, keys, k0, k1;
+    list_extent(a, ls, list, r0, r1, keys);
+    part_range(keys, ls.splits, split, k0, k1);
+    const int n_rows = (r1 - r0) * G;
+    const T* kp = reinterpret_cast<const T*>(a.kp);
+    const T* vp = reinterpret_cast<const T*>(a.vp);
+
+    for (int t0 = tile0 * 16; t0 < n_rows; t0 += row_tiles * 16) {
+        const int mine = t0 + (lane & 15);                 // (row, head) pair of this lane
+        const bool live = mine < n_rows;
+        const int row = r0 + (live ? mine / G : 0);
+        const int head = hk * G + (live ? mine % G : 0);
+        // keys that this row and the tile's first row see (later rows see no fewer)
+        const int limit = ls.causal ? keys - (r1 - row) + 1 : keys;
+        const int first_limit = ls.causal ? keys - (r1 - r0 - t0 / G) + 1 : keys;
+        const int last_limit = ls.causal ? keys - (r1 - r0 - min(t0 + 15, n_rows - 1) / G) + 1 : keys;
+        const int end = min(k1, last_limit);
+
+        Tile t;
+        t.load_q(reinterpret_cast<const T*>(a.q) + (int64_t)row * a.q_row + (int64_t)head * a.q_head, live, lane);
+        f32x4_t o[Tile::kO];
+#pragma unroll
+        for (int c = 0; c < Tile::kO; ++c) o[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        bool seen = false;
+
+        // place of the 16 keys from `key` on: element offset of the first, and how many of them there are
+        auto place = [&](int key, size_t& off, int& there) {
+            const int page = key < end ? ls.table.page(list, key) : -1;
+            there = page >= 0 ? min(16, end - key) : 0;
+            off = page >= 0 ? ((((size_t)page * a.hk + hk) << ls.table.page_shift) + (key & ((1 << ls.table.page_shift) - 1))) * D : 0;
+        };
+        size_t off[2], off_next[2];
+        int there[2], there_next[2];
+        int key = k0 + wave * Tile::kKeys;
+#pragma unroll
+        for (int h = 0; h < Tile::kHalves; ++h) {
+            place(key + 16 * h, off[h], there[h]);
+            if (key < end) t.load_k(h, kp + off[h], lane);
+        }
+        for (; key < end; key += 4 * Tile::kKeys) {
+            // the values of this group and the keys of the next are in flight while the scores are worked out
+#pragma unroll
+            for (int h = 0; h < Tile::kHalves; ++h) t.load_v(h, vp + off[h], lane);
+            const int next = key + 4 * Tile::kKeys;
+#pragma unroll
+            for (int h = 0; h < Tile::kHalves; ++h) place(next + 16 * h, off_next[h], there_next[h]);
+            float s[NP];
+            t.scores(s);
+            if (next < end) {
+#pragma unroll
+                for (int h = 0; h < Tile::kHalves; ++h) t.load_k(h, kp + off_next[h], lane);
             }
-            s += __shfl_xor(s, 1, 64);
-            s += __shfl_xor(s, 2, 64);
-            seen = true;
-            const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-            const float alpha = exp2f((m - ref) * a.scale_log2), p = exp2f((s - ref) * a.scale_log2);
-            l = l * alpha + p;
+            bool whole = key + Tile::kKeys <= first_limit;  // every row sees every key of the group
 #pragma unroll
-            for (int i = 0; i < P; ++i)
+            for (int h = 0; h < Tile::kHalves; ++h) whole = whole && there[h] == 16;
+            bool apart = false;                             // a hidden value is not finite: a product with 0 would show it
+            if (whole) {
+                seen = true;
+            } else {
 #pragma unroll
-                for (int t = 0; t < 8; ++t) acc[i][t] = acc[i][t] * alpha + p * vv[i][t];
-            m = mn;
+                for (int h = 0; h < Tile::kHalves; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 4 * quad + e;
+                        const bool here = i < there[h], vis = here && key + 16 * h + i < limit;
+                        if (!vis) s[4 * h + e] = -INFINITY;
+                        seen |= vis;
+                        if (!here) t.clear_v(h, e);
+                        else if (key + 16 * h + i >= first_limit) apart |= t.v_not_finite(h, e);
+                    }
+            }
+            float top = s[0];
+#pragma unroll
+            for (int i = 1; i < NP; ++i) top = fmaxf(top, s[i]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (__any(top > m)) {                           // else the running maxima stand and nothing is scaled
+                const float mn = fmaxf(m, top);
+                const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+                m = mn;
+                l *= w;
+#pragma unroll
+                for (int c = 0; c < Tile::kO; ++c) o[c] *= w;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+            float p[NP];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                p[i] = __builtin_amdgcn_exp2f((s[i] - ref) * a.scale_log2);
+                l += p[i];
+            }
+            if (__any(apart)) {
+                // what is not finite goes one key at a time into the rows that see it; the rest of the group as ever
+#pragma unroll 1
+                for (int i = 0; i < Tile::kKeys; ++i) t.weigh_not_finite(p, o, i, key + i < limit, lane);
+                t.clear_not_finite();
+            }
+            t.weigh(p, o);
+#pragma unroll
+            for (int h = 0; h < Tile::kHalves; ++h) {
+                off[h] = off_next[h];
+                there[h] = there_next[h];
+            }
         }
-    };
-    if (prefix > 0) walk(a.prefix_table, group, prefix);
-    walk(a.table, seq, keys);
-    float M = m;
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        int any = seen ? 1 : 0;
+        any |= __shfl_xor(any, 16, 64);
+        any |= __shfl_xor(any, 32, 64);
+        // m: -inf only where no key was seen; keys that all score -inf leave l = 0, and 0 / 0 as the formula has it
+        if (any && m == -INFINITY) m = -FLT_MAX;
 #pragma unroll
-    for (int off = 4; off <= 32; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
-    const float f = seen ? exp2f((m - (M == -INFINITY ? 0.f : M)) * a.scale_log2) : 0.f;
-    float L = l * f;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int off = 4; off <= 32; off <<= 1) L += __shfl_xor(L, off, 64);
-    const bool any = __any(seen);                  // a row that sees no key gives zeros; 0 / 0 elsewhere is the formula's
+            for (int c = 0; c < Tile::kO; ++c) red_o[wave][lane & 15][Tile::dim(c, r, lane)] = o[c][r];
+        if (quad == 0) red_ml[wave][lane & 15] = make_float2(m, l);
+        __syncthreads();
+        const int tile_rows = min(16, n_rows - t0);
+        for (int i = threadIdx.x; i < tile_rows * (D / 4); i += 256) {
+            const int x = i / (D / 4), d4 = i % (D / 4) * 4;
+            float M = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, red_ml[w][x].x);
+            float L = 0.f;
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            float x = acc[i][t] * f;
+            for (int w = 0; w < 4; ++w) {
+                const float2 ml = red_ml[w][x];
+                const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * a.scale_log2);
+                L += ml.y * f;
+                acc += *reinterpret_cast<const f32x4_t*>(&red_o[w][x][d4]) * f;
+            }
+            const size_t at = (size_t)(r0 + (t0 + x) / G) * a.hq + hk * G + (t0 + x) % G;
+            if (a.part_o) {
+                const size_t part = (size_t)(ls.part0 + split) * ((size_t)a.rows * a.hq) + at;
+                *reinterpret_cast<f32x4_t*>(a.part_o + part * D + d4) = acc;
+                if (d4 == 0) a.part_ml[part] = make_float2(M, L);
+            } else {
+                T* dst = reinterpret_cast<T*>(a.out) + at * D + d4;
 #pragma unroll
-            for (int off = 4; off <= 32; off <<= 1) x += __shfl_xor(x, off, 64);
-            acc[i][t] = any ? x / L : 0.f;
+                for (int e = 0; e < 4; ++e) Elem<T>::store(dst + e, M == -INFINITY ? 0.f : acc[e] / L);
+            }
         }
-        if (ks == 0) store8<T>(reinterpret_cast<T*>(a.out) + ((size_t)row * a.hq + head) * D + col + 32 * i, acc[i]);
+        __syncthreads();
+    }
+}
+
+struct JoinArgs {
+    int parts, prefix_parts;         // the prefix's parts come first
+    const int32_t* group_starts;     // null: no prefix
+    int n_groups;
+};
+
+// Joins the parts of every (row, head): D / 4 lanes each, which hold the statistics of the parts between them.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, JoinArgs j) {
+    constexpr int L4 = D / 4;
+    const int64_t at = (int64_t)blockIdx.x * (256 / L4) + threadIdx.x / L4;
+    const int sub = threadIdx.x % L4;
+    const int64_t row = at / a.hq;
+    // rows of no sequence are left alone; those of no group have no prefix
+    const int first = a.q_starts ? a.q_starts[0] : 0, last = a.q_starts ? a.q_starts[a.n_seqs] : a.n_seqs;
+    const bool live = row < a.rows && row >= first && row < last;
+    int part0 = j.prefix_parts;
+    if (j.group_starts) {
+        const int s0 = min(max(j.group_starts[0], 0), a.n_seqs), s1 = min(max(j.group_starts[j.n_groups], 0), a.n_seqs);
+        if (row >= (a.q_starts ? a.q_starts[s0] : s0) && row < (a.q_starts ? a.q_starts[s1] : s1)) part0 = 0;
+    }
+    const int64_t stride = (int64_t)a.rows * a.hq;
+    float M = -INFINITY;
+    for (int p = part0 + sub; p < j.parts; p += L4)
+        if (live) M = fmaxf(M, a.part_ml[p * stride + at].x);
+#pragma unroll
+    for (int off = L4 / 2; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+    float L = 0.f;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = part0; p0 < j.parts; p0 += L4) {
+        const int p = p0 + sub;
+        float w = 0.f;
+        if (live && p < j.parts) {
+            const float2 ml = a.part_ml[p * stride + at];
+            if (ml.x != -INFINITY) {
+                w = __builtin_amdgcn_exp2f((ml.x - M) * a.scale_log2);
+                L += ml.y * w;
+            }
+        }
+        const int n = min(L4, j.parts - p0);
+        for (int i = 0; i < n; ++i) {
+            const float f = __shfl(w, i, L4);
+            if (f > 0.f) acc += *reinterpret_cast<const f32x4_t*>(a.part_o + ((p0 + i) * stride + at) * D + 4 * sub) * f;
+        }
+    }
+#pragma unroll
+    for (int off = L4 / 2; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
+    if (live) {
+        T* dst = reinterpret_cast<T*>(a.out) + at * D + 4 * sub;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) Elem<T>::store(dst + e, M == -INFINITY ? 0.f : acc[e] / L);
     }
 }
 
@@ -116,6 +491,60 @@ static int check_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     return LCMHIP_OK;
 }
 
+// How a call is cut: parts of the own keys and of the prefix.  One workgroup walks one part for one key head and 16 rows; parts
+// are added until the grid has kWanted workgroups, and none is shorter than kMinPart.
+constexpr int kWanted = 2048, kMaxParts = 64;
+struct Plan {
+    int own_splits = 1, prefix_splits = 0, own_tiles = 1, prefix_tiles = 1;
+    bool joined = false;
+    int64_t part_rows = 0;
+    size_t ml_bytes = 0, bytes = 0;
+};
+
+static int splits_for(int64_t blocks, int max_keys) {
+    const int64_t most = std::min<int64_t>(kMaxParts, (max_keys + kMinPart - 1) / kMinPart);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(most, kWanted / std::max<int64_t>(blocks, 1)));
+}
+
+static Plan make_plan(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, const lcmhip_shared_prefix* prefix, int64_t rows,
+                      int n_heads) {
+    Plan p;
+    const int G = n_heads / pages->n_kv_heads;
+    p.own_tiles = (int)std::min<int64_t>(((int64_t)batch->max_q * G + 15) / 16, (rows * G + 15) / 16);
+    p.own_splits = splits_for((int64_t)batch->n_seqs * pages->n_kv_heads * p.own_tiles, batch->max_keys);
+    if (prefix) {
+        p.prefix_tiles = (int)((rows * G + 15) / 16);
+        p.prefix_splits = splits_for((int64_t)pages->n_kv_heads * (p.prefix_tiles + prefix->n_groups), prefix->max_keys);
+    }
+    p.joined = p.own_splits + p.prefix_splits > 1;
+    if (p.joined) {
+        const size_t n = (size_t)(p.own_splits + p.prefix_splits) * rows * n_heads;
+        p.ml_bytes = (n * sizeof(float2) + 255) & ~(size_t)255;
+        p.bytes = p.ml_bytes + n * pages->head_dim * sizeof(float);
+    }
+    return p;
+}
+
+template <typename T, int D>
+static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists& prefix, const Plan& p, hipStream_t st) {
+    auto few = [&](const KeyLists& ls, int tiles) {
+        const int64_t blocks = (int64_t)a.hk * ls.splits * ls.n * tiles;
+        LCM_REQUIRE(blocks <= INT32_MAX, "paged attention: too many rows");
+        hipLaunchKernelGGL((k_paged_few<T, D>), dim3((unsigned)blocks), dim3(256), 0, st, a, ls, tiles);
+        LCM_HIP_CHECK(hipGetLastError());
+        return LCMHIP_OK;
+    };
+    if (prefix.n > 0) LCM_TRY(few(prefix, p.prefix_tiles));
+    LCM_TRY(few(own, p.own_tiles));
+    if (p.joined) {
+        const int64_t per = 256 / (D / 4);
+        hipLaunchKernelGGL((k_paged_join<T, D>), dim3((unsigned)(((int64_t)a.rows * a.hq + per - 1) / per)), dim3(256), 0, st, a,
+                           JoinArgs{p.own_splits + p.prefix_splits, p.prefix_splits, prefix.group_starts, prefix.n});
+        LCM_HIP_CHECK(hipGetLastError());
+    }
+    return LCMHIP_OK;
+}
+
 static int paged_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, const lcmhip_shared_prefix* prefix,
                            const void* q, int64_t q_row, int64_t q_head, void* out, int64_t rows, int n_heads, float scale,
                            int causal, void* ws, size_t ws_bytes, hipStream_t st) {
@@ -126,27 +555,26 @@ static int paged_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     LCM_TRY(check_rows(q, q_row, q_head, pages->dtype, "paged attention: q"));
     LCM_TRY(check_rows(out, 0, 0, pages->dtype, "paged attention: out"));
     if (rows == 0 || batch->n_seqs == 0) return LCMHIP_OK;
+    const Plan p = make_plan(pages, batch, prefix, rows, n_heads);
+    LCM_REQUIRE(ws_bytes >= p.bytes && (p.bytes == 0 || (ws && (uintptr_t)ws % 256 == 0)),
+                "paged attention: workspace too small, missing or not 256-byte aligned");
     PagedArgs a{};
     a.q = q; a.q_row = q_row; a.q_head = q_head; a.out = out; a.kp = pages->k; a.vp = pages->v;
-    a.table = PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), pages->n_pages};
-    a.seq_lens = batch->seq_lens; a.q_starts = batch->q_starts; a.n_seqs = batch->n_seqs; a.max_keys = batch->max_keys;
-    if (prefix) {
-        a.prefix_table = PageTable{prefix->page_table, prefix->max_pages, page_shift_of(pages), pages->n_pages};
-        a.prefix_lens = prefix->lens; a.group_starts = prefix->group_starts;
-        a.n_groups = prefix->n_groups; a.prefix_max_keys = prefix->max_keys;
-    }
-    a.rows = rows; a.hq = n_heads; a.hk = pages->n_kv_heads; a.causal = causal;
+    a.q_starts = batch->q_starts; a.n_seqs = batch->n_seqs;
+    a.rows = (int)rows; a.hq = n_heads; a.hk = pages->n_kv_heads;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const dim3 grid((unsigned)(rows * n_heads)), block(64);
-    if (pages->dtype == LCMHIP_BF16) {
-        if (pages->head_dim == 64) hipLaunchKernelGGL((k_paged_rows<bf16_t, 64>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((k_paged_rows<bf16_t, 128>), grid, block, 0, st, a);
-    } else {
-        if (pages->head_dim == 64) hipLaunchKernelGGL((k_paged_rows<float, 64>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((k_paged_rows<float, 128>), grid, block, 0, st, a);
+    const KeyLists own{PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), pages->n_pages}, batch->seq_lens, nullptr,
+                     batch->n_seqs, batch->max_keys, causal != 0, p.own_splits, p.prefix_splits};
+    KeyLists pre{};
+    if (prefix)
+        pre = KeyLists{PageTable{prefix->page_table, prefix->max_pages, page_shift_of(pages), pages->n_pages}, prefix->lens,
+                            prefix->group_starts, prefix->n_groups, prefix->max_keys, 0, p.prefix_splits, 0};
+    if (p.joined) {
+        a.part_ml = reinterpret_cast<float2*>(ws);
+        a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + p.ml_bytes);
     }
-    LCM_HIP_CHECK(hipGetLastError());
-    return LCMHIP_OK;
+    if (pages->dtype == LCMHIP_BF16) return pages->head_dim == 64 ? launch_paged<bf16_t, 64>(a, own, pre, p, st) : launch_paged<bf16_t, 128>(a, own, pre, p, st);
+    return pages->head_dim == 64 ? launch_paged<float, 64>(a, own, pre, p, st) : launch_paged<float, 128>(a, own, pre, p, st);
 }
 
 }  // namespace lcmhip
@@ -159,7 +587,7 @@ int lcmhip_paged_attention_workspace(const lcmhip_kv_pages* pages, const lcmhip_
                                      size_t* bytes) {
     LCM_REQUIRE(bytes, "paged_attention_workspace: null argument");
     LCM_TRY(check_attention(pages, batch, rows, n_heads));
-    *bytes = 0;
+    *bytes = make_plan(pages, batch, nullptr, rows, n_heads).bytes;
     return LCMHIP_OK;
 }
 
@@ -175,7 +603,7 @@ int lcmhip_shared_prefix_attention_workspace(const lcmhip_kv_pages* pages, const
     LCM_REQUIRE(bytes, "shared_prefix_attention_workspace: null argument");
     LCM_TRY(check_attention(pages, batch, rows, n_heads));
     LCM_TRY(check_prefix(pages, prefix));
-    *bytes = 0;
+    *bytes = make_plan(pages, batch, prefix, rows, n_heads).bytes;
     return LCMHIP_OK;
 }
 
