@@ -27,6 +27,7 @@ from lcm import _hip
 from lcm.nn.normalization import norm_kind
 
 _lib = _hip.lib
+_NO_BACKWARD = "the paged cache operators have no backward: call them under torch.no_grad() or detach the inputs"
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -83,11 +84,11 @@ class HeadNorm:
         self._c = _hip.HeadNorm(*(None if t is None else t.data_ptr() for t in self.tensors), norm_kind(kind), self.eps)
         self._ref = C.byref(self._c)
 
-    def _check(self, head_dim: int, like: Tensor) -> None:
-        if self._like is not None:
-            _require(self._like == (head_dim, like.dtype, like.device), f"head norm weights are {self._like}, the heads "
-                     f"{(head_dim, like.dtype, like.device)}")
-            _grad_free(*(t for t in self.tensors if t is not None))
+    def _check(self, head_dim: int, dtype: torch.dtype, device: torch.device) -> None:
+        if self._like is not None and self._like != (head_dim, dtype, device):
+            raise ValueError(f"head norm weights are {self._like}, the heads {(head_dim, dtype, device)}")
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in self.tensors):
+            raise RuntimeError(_NO_BACKWARD)
 
 
 class KVPages:
@@ -139,15 +140,11 @@ class PagedBatch:
     def _bind(self, pages: KVPages, rows: int):
         """The C struct with max_keys filled in for this page size."""
         if self._fit != pages.page_size:
-            reach = self.max_pages * pages.page_size
-            if self.max_keys is None:
-                self._c.max_keys = min(reach, 2**31 - 1)
-            else:
-                _require(1 <= self.max_keys <= reach, f"max_keys {self.max_keys} is not in [1, {reach}], what the page table holds")
-                self._c.max_keys = self.max_keys
-            self._fit = pages.page_size
-        _require(self.device == pages.device, f"the batch lives on {self.device}, the pages on {pages.device}")
-        _require(self.q_starts is not None or rows == self.num_seqs, "without q_starts there is one row for every sequence")
+            self._c.max_keys, self._fit = _reach(self.max_keys, self.max_pages, pages), pages.page_size
+        if self.device != pages.device:
+            raise ValueError(f"the batch lives on {self.device}, the pages on {pages.device}")
+        if self.q_starts is None and rows != self.num_seqs:
+            raise ValueError("without q_starts there is one row for every sequence")
         return self._ref
 
 
@@ -171,55 +168,67 @@ class SharedPrefix:
 
     def _bind(self, pages: KVPages):
         if self._fit != pages.page_size:
-            reach = self.max_pages * pages.page_size
-            if self.max_keys is None:
-                self._c.max_keys = min(reach, 2**31 - 1)
-            else:
-                _require(1 <= self.max_keys <= reach, f"max_keys {self.max_keys} is not in [1, {reach}], what the page table holds")
-                self._c.max_keys = self.max_keys
-            self._fit = pages.page_size
-        _require(self.device == pages.device, f"the prefix lives on {self.device}, the pages on {pages.device}")
+            self._c.max_keys, self._fit = _reach(self.max_keys, self.max_pages, pages), pages.page_size
+        if self.device != pages.device:
+            raise ValueError(f"the prefix lives on {self.device}, the pages on {pages.device}")
         return self._ref
+
+
+def _reach(max_keys: Optional[int], max_pages: int, pages: KVPages) -> int:
+    reach = max_pages * pages.page_size
+    if max_keys is None:
+        return min(reach, 2**31 - 1)
+    if not 1 <= max_keys <= reach:
+        raise ValueError(f"max_keys {max_keys} is not in [1, {reach}], what the page table holds")
+    return max_keys
 
 
 def _grad_free(*tensors: Tensor) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
-                raise RuntimeError("the paged cache operators have no backward: call them under torch.no_grad() or detach the inputs")
+                raise RuntimeError(_NO_BACKWARD)
 
 
-def _heads(t: Tensor, what: str, like: Optional[Tensor] = None, heads: Optional[int] = None, head_dim: Optional[int] = None) -> Tuple[int, int, int]:
-    """(pointer, row stride, head stride) of a row tensor (rows, heads, head_dim) with a dense last dimension."""
-    _hip.require_gpu(t, what)
-    _require(t.dim() == 3 and t.stride(2) == 1, f"{what} must be (rows, heads, head_dim) with a dense last dimension")
-    if like is not None:
-        _require(t.dtype == like.dtype and t.device == like.device and t.shape[0] == like.shape[0] and t.shape[2] == like.shape[2],
-                 f"{what} does not match: {tuple(t.shape)} {t.dtype} {t.device} beside {tuple(like.shape)} {like.dtype} {like.device}")
-    _require(heads is None or t.shape[1] == heads, f"{what} has {t.shape[1]} heads, not {heads}")
-    _require(head_dim is None or t.shape[2] == head_dim, f"{what} has heads of {t.shape[2]}, not {head_dim}")
+def _heads(t: Tensor, what: str, dtype: torch.dtype, device: torch.device, rows: Optional[int], heads: Optional[int],
+           head_dim: int) -> Tuple[int, int, int]:
+    """(pointer, row stride, head stride) of a row tensor (rows, heads, head_dim) with a dense last dimension; None: any number.
+    These checks stand in front of kernels of a few microseconds: they build no message before they fail."""
+    shape = t.shape
+    if len(shape) != 3 or t.stride(2) != 1 and shape[2] != 1:
+        raise ValueError(f"{what} must be (rows, heads, head_dim) with a dense last dimension")
+    if t.device != device:
+        _hip.require_gpu(t, what)
+        raise ValueError(f"{what} lives on {t.device}, not on {device}")
+    if (t.dtype is not dtype or shape[2] != head_dim or (heads is not None and shape[1] != heads)
+            or (rows is not None and shape[0] != rows)):
+        raise ValueError(f"{what} is {tuple(shape)} {t.dtype}, expected ({'any' if rows is None else rows}, "
+                         f"{'any' if heads is None else heads}, {head_dim}) {dtype}")
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
 def _call(device: torch.device, fn, *args) -> None:
     """Runs a library entry point on the current stream of `device`."""
-    if torch.cuda.current_device() == device.index:
-        _hip.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        _hip.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
-        with torch.cuda.device(device):
-            _hip.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            _hip.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _transform(rope: Optional[RotaryTable], norm: Optional[HeadNorm], positions: Optional[Tensor], like: Tensor):
-    head_dim = like.shape[2]
+    rows, _, head_dim = like.shape
+    device = like.device
     if norm is not None:
-        norm._check(head_dim, like)
-    if rope is not None:
-        _require(rope.device == like.device, f"the rotary table lives on {rope.device}, not on {like.device}")
+        norm._check(head_dim, like.dtype, device)
+    if rope is not None and rope.device != device:
+        raise ValueError(f"the rotary table lives on {rope.device}, not on {device}")
     pos = None
     if positions is not None:
-        pos = _index(positions, "positions", 1, like.device)
-        _require(positions.shape[0] == like.shape[0], "positions must have one entry for every row")
+        if positions.dtype is not torch.int32 or positions.shape != (rows,) or positions.device != device or not positions.is_contiguous():
+            raise ValueError(f"positions must be a contiguous int32 tensor with one entry for every row on {device}")
+        pos = positions.data_ptr()
     return None if norm is None else norm._ref, None if rope is None else rope._ref, pos
 
 
@@ -233,29 +242,37 @@ def head_norm_rope(q: Optional[Tensor], k: Optional[Tensor], *, positions: Optio
     like = q if q is not None else k
     _require(like is not None, "head_norm_rope needs queries or keys")
     _hip.require_gpu(like, "heads")
-    args, outs = [], []
-    for x, out, what in ((q, q_out, "q"), (k, k_out, "k")):
-        if x is None:
-            _require(out is None, f"{what}_out without {what}")
-            args.append((None, 0, 0))
-            outs.append((None, 0, 0))
-            continue
-        _grad_free(x)
-        args.append(_heads(x, what, like))
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            if what == "q":
-                q_out = out
-            else:
-                k_out = out
-        outs.append(_heads(out, what + "_out", x, x.shape[1]))
+    dtype, device = like.dtype, like.device
+    _require(like.dim() == 3, "queries and keys must be (rows, heads, head_dim)")
+    rows, _, head_dim = like.shape
+    q_args = k_args = qo_args = ko_args = (None, 0, 0)
+    q_heads = k_heads = 0
+    if q is not None:
+        _grad_free(q)
+        q_args, q_heads = _heads(q, "q", dtype, device, rows, None, head_dim), q.shape[1]
+        if q_out is None:
+            q_out = q.new_empty(q.shape)
+            qo_args = q_out.data_ptr(), q_heads * head_dim, head_dim
+        else:
+            qo_args = _heads(q_out, "q_out", dtype, device, rows, q_heads, head_dim)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if k is not None:
+        _grad_free(k)
+        k_args, k_heads = _heads(k, "k", dtype, device, rows, None, head_dim), k.shape[1]
+        if k_out is None:
+            k_out = k.new_empty(k.shape)
+            ko_args = k_out.data_ptr(), k_heads * head_dim, head_dim
+        else:
+            ko_args = _heads(k_out, "k_out", dtype, device, rows, k_heads, head_dim)
+    elif k_out is not None:
+        raise ValueError("k_out without k")
     _require(rope is None or positions is not None, "a rotation needs positions")
     norm_ref, rope_ref, pos = _transform(rope, norm, positions, like)
-    if like.shape[0] == 0:                 # an empty tensor has no address
+    if rows == 0:                          # an empty tensor has no address
         return q_out, k_out
-    _call(like.device, _lib.lcmhip_head_norm_rope, *args[0], *args[1], *outs[0], *outs[1], like.shape[0],
-          0 if q is None else q.shape[1], 0 if k is None else k.shape[1], like.shape[2], norm_ref, rope_ref, pos,
-          _hip.dtype_code(like.dtype))
+    _call(device, _lib.lcmhip_head_norm_rope, *q_args, *k_args, *qo_args, *ko_args, rows, q_heads, k_heads, head_dim, norm_ref,
+          rope_ref, pos, _hip.dtype_code(dtype))
     return q_out, k_out
 
 
@@ -270,51 +287,53 @@ def paged_append(pages: KVPages, batch: PagedBatch, k: Tensor, v: Tensor, *, q: 
     `positions` is None.  Rows without a place (before the sequence's beginning, behind its table, of no sequence, or of a
     negative position) are skipped."""
     _grad_free(k, v)
-    kp = _heads(k, "k", None, pages.num_kv_heads, pages.head_dim)
-    vp = _heads(v, "v", k, pages.num_kv_heads)
-    _require(k.dtype == pages.dtype and k.device == pages.device, f"k is {k.dtype} on {k.device}, the pages {pages.dtype} on {pages.device}")
+    dtype, device, head_dim, kv_heads = pages.dtype, pages.device, pages.head_dim, pages.num_kv_heads
+    kp = _heads(k, "k", dtype, device, None, kv_heads, head_dim)
+    rows = k.shape[0]
+    vp = _heads(v, "v", dtype, device, rows, kv_heads, head_dim)
     qp, heads, qo = (None, 0, 0), 0, None
     if q is not None:
         _grad_free(q)
-        qp, heads = _heads(q, "q", k), q.shape[1]
+        qp, heads = _heads(q, "q", dtype, device, rows, None, head_dim), q.shape[1]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = q.new_empty(q.shape)
         else:
-            _heads(q_out, "q_out", q, heads)
+            _heads(q_out, "q_out", dtype, device, rows, heads, head_dim)
             _require(q_out.is_contiguous(), "q_out must be contiguous")
         qo = q_out.data_ptr()
-    else:
-        _require(q_out is None, "q_out without q")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
     norm_ref, rope_ref, pos = _transform(rope, norm, positions, k)
-    if k.shape[0] == 0:
-        return q_out
-    _call(k.device, _lib.lcmhip_paged_append, pages._ref, batch._bind(pages, k.shape[0]), *kp, *vp, *qp, qo, k.shape[0], heads,
-          norm_ref, rope_ref, pos)
+    batch_ref = batch._bind(pages, rows)
+    if rows:
+        _call(device, _lib.lcmhip_paged_append, pages._ref, batch_ref, *kp, *vp, *qp, qo, rows, heads, norm_ref, rope_ref, pos)
     return q_out
 
 
 def _attend(q: Tensor, pages: KVPages, batch: PagedBatch, prefix: Optional[SharedPrefix], causal: bool, scale: Optional[float],
             out: Optional[Tensor]) -> Tensor:
     _grad_free(q)
-    qp = _heads(q, "q", None, None, pages.head_dim)
-    rows, heads = q.shape[0], q.shape[1]
-    _require(q.dtype == pages.dtype and q.device == pages.device, f"q is {q.dtype} on {q.device}, the pages {pages.dtype} on {pages.device}")
+    qp = _heads(q, "q", pages.dtype, pages.device, None, None, pages.head_dim)
+    rows, heads, head_dim = q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     else:
-        _heads(out, "out", q, heads)
+        _heads(out, "out", pages.dtype, pages.device, rows, heads, head_dim)
         _require(out.is_contiguous(), "out must be contiguous")
-    refs = (pages._ref, batch._bind(pages, rows)) + (() if prefix is None else (prefix._bind(pages),))
+    if prefix is None:
+        refs, fn, size_fn = (pages._ref, batch._bind(pages, rows)), _lib.lcmhip_paged_attention, _lib.lcmhip_paged_attention_workspace
+    else:
+        refs, fn, size_fn = ((pages._ref, batch._bind(pages, rows), prefix._bind(pages)), _lib.lcmhip_shared_prefix_attention,
+                             _lib.lcmhip_shared_prefix_attention_workspace)
     if rows == 0:
         return out
     need = C.c_size_t()
-    size_fn = _lib.lcmhip_paged_attention_workspace if prefix is None else _lib.lcmhip_shared_prefix_attention_workspace
     _hip.check(size_fn(*refs, rows, heads, C.byref(need)))
+    size = need.value
     # partial results live as long as the call's kernels: the allocator orders the memory's next use behind them
-    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-    fn = _lib.lcmhip_paged_attention if prefix is None else _lib.lcmhip_shared_prefix_attention
-    _call(q.device, fn, *refs, *qp, out.data_ptr(), rows, heads, pages.head_dim ** -0.5 if scale is None else scale, int(causal),
-          None if ws is None else ws.data_ptr(), need.value)
+    ws = q.new_empty(size, dtype=torch.uint8) if size else None
+    _call(pages.device, fn, *refs, *qp, out.data_ptr(), rows, heads, head_dim ** -0.5 if scale is None else scale, int(causal),
+          None if ws is None else ws.data_ptr(), size)
     return out
 
 
