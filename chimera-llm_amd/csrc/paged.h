@@ -5,18 +5,26 @@
 
 namespace lcmhip {
 
+// An index that no kernel of the call writes, read through the scalar path where its address is the same for a wave.
+__host__ __device__ __forceinline__ int32_t read_index(const int32_t* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+#else
+    return *p;
+#endif
+}
+
 // A table of page ids as the kernels see it.  Nothing in the index arrays is trusted with an address: page() answers -1
 // for an id outside the pool and for a position behind the table.
 struct PageTable {
     const int32_t* ids;
     int max_pages;
     int page_shift;          // log2(page_size)
-    int64_t n_pages;
-    __host__ __device__ __forceinline__ int page(int seq, int pos) const {
+    uint32_t n_pages;
+    __host__ __device__ __forceinline__ int page(int seq, int pos) const {   // pos >= 0
         const int p = pos >> page_shift;
-        if (p >= max_pages) return -1;
-        const int id = ids[(size_t)seq * max_pages + p];
-        return id >= 0 && id < n_pages ? id : -1;
+        const int32_t id = read_index(ids + ((size_t)seq * max_pages + (p < max_pages ? p : max_pages - 1)));
+        return p < max_pages && (uint32_t)id < n_pages ? id : -1;
     }
 };
 

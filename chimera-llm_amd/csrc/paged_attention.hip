@@ -45,14 +45,14 @@ struct PagedArgs {
 __device__ __forceinline__ void list_extent(const PagedArgs& a, const KeyLists& ls, int i, int& r0, int& r1, int& keys) {
     int s0 = i, s1 = i + 1;
     if (ls.group_starts) {
-        s0 = min(max(ls.group_starts[i], 0), a.n_seqs);
-        s1 = min(max(ls.group_starts[i + 1], s0), a.n_seqs);
+        s0 = min(max(read_index(ls.group_starts + i), 0), a.n_seqs);
+        s1 = min(max(read_index(ls.group_starts + i + 1), s0), a.n_seqs);
     }
-    r0 = a.q_starts ? a.q_starts[s0] : s0;
-    r1 = a.q_starts ? a.q_starts[s1] : s1;
+    r0 = a.q_starts ? read_index(a.q_starts + s0) : s0;
+    r1 = a.q_starts ? read_index(a.q_starts + s1) : s1;
     r0 = min(max(r0, 0), a.rows);
     r1 = min(max(r1, r0), a.rows);
-    keys = max(0, min(ls.lens[i], ls.max_keys));
+    keys = max(0, min(read_index(ls.lens + i), ls.max_keys));
 }
 
 // Part `split` of `keys` keys: at most `splits` equal parts, multiples of 32 keys, of no fewer than kMinPart.
@@ -419,6 +419,399 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedArgs a, KeyLists ls, 
     }
 }
 
+// ---- a tile of 32 rows against tiles of keys in LDS, by one wave -----------------------------------------------------------------
+// The same two products on 32 x 32 matrix instructions; lane = row lane % 32, hi = lane / 32:
+//     S^T  register r of a 32-key block holds key 8 (r / 4) + 4 hi + r % 4
+//     O^T  register r of dim block t holds row 8 (r / 4) + 4 hi + r % 4 of the block
+// Keys and values lie row-major in LDS, 16-byte pieces permuted inside a row (piece ^ swizzle(row)) so that the pieces one
+// instruction reads from different rows lie in different banks; LDS-DMA fills a row's pieces in that order.
+using f32x16_t = __attribute__((ext_vector_type(16))) float;
+using s16x4_t = __attribute__((ext_vector_type(4))) short;
+typedef const __attribute__((address_space(1))) void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_t;
+
+template <typename T, int D>
+struct Tile32;
+
+template <int D>
+struct Tile32<bf16_t, D> {
+    static constexpr int kKeys = 64, kRow = 2 * D, kO = D / 32;
+    bf16x8_t q[D / 16];
+    int k_off, v_off[2];                                   // LDS byte offsets of this lane inside a tile, before the step's XOR
+
+    // D = 128: a row is all 64 banks, so four consecutive rows go to four different quarters for the 8-byte transposed reads and
+    // sixteen to sixteen pieces for the 16-byte reads.  D = 64: two rows are all banks.
+    __device__ static __forceinline__ int swizzle(int row) {
+        return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    }
+    __device__ __forceinline__ void init(int lane) {
+        const int c = lane & 31, hi = lane >> 5, i = lane & 15, dh = (lane >> 4) & 1;
+        k_off = c * kRow + ((hi ^ swizzle(c)) << 4);       // piece 2 st + hi of row c: ^ (st << 5)
+#pragma unroll
+        for (int sec = 0; sec < 2; ++sec) {                // value rows 4 hi + i / 4 (+ 8), dims 16 dh + 4 (i % 4) ..: ^ (t << 6)
+            const int row = 8 * sec + 4 * hi + (i >> 2);
+            v_off[sec] = row * kRow + (((2 * dh + ((i & 3) >> 1)) ^ swizzle(row)) << 4) + 8 * (i & 1);
+        }
+    }
+    // Keeps the offsets of all steps, one XOR each, from being worked out before the loop and held in registers.
+    __device__ __forceinline__ void fresh_offsets() { asm volatile("" : "+v"(k_off), "+v"(v_off[0]), "+v"(v_off[1])); }
+    __device__ __forceinline__ void load_q(const bf16_t* row, bool live, int lane) {
+#pragma unroll
+        for (int st = 0; st < D / 16; ++st) {
+            u32x4_t x = {0, 0, 0, 0};
+            if (live) x = *reinterpret_cast<const u32x4_t*>(row + 16 * st + 8 * (lane >> 5));
+            q[st] = __builtin_bit_cast(bf16x8_t, x);
+        }
+    }
+    __device__ __forceinline__ f32x16_t scores(const char* ks, int kb) const {
+        f32x16_t s = {};
+#pragma unroll
+        for (int st = 0; st < D / 16; ++st) {
+            const bf16x8_t k = *reinterpret_cast<const bf16x8_t*>(ks + kb * 32 * kRow + (k_off ^ (st << 5)));
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[st], s, 0, 0, 0);
+        }
+        return s;
+    }
+    __device__ __forceinline__ bf16x8_t v_operand(const char* vs, int kb, int u, int t) const {
+        const char* base = vs + (kb * 32 + u * 16) * kRow;
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(base + (v_off[0] ^ (t << 6))));
+        const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(base + (v_off[1] ^ (t << 6))));
+        return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    // o += P V for a 32-key block; probabilities are rounded to bf16 as in Tile16
+    __device__ __forceinline__ static bf16x8_t p_operand(const f32x16_t& p, int u) {
+        bf16x8_t pf;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pf[e] = (__bf16)p[8 * u + e];
+        return pf;
+    }
+    __device__ __forceinline__ void weigh(const char* vs, int kb, const f32x16_t& p, f32x16_t (&o)[kO]) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bf16x8_t pf = p_operand(p, u);
+#pragma unroll
+            for (int t = 0; t < kO; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_operand(vs, kb, u, t), pf, o[t], 0, 0, 0);
+        }
+    }
+    // Infinities and NaNs of a block's values for the rows that see them (bit r of `sees`: the key of register r): counted by a
+    // product of ones, in which nothing can leave its row.
+    __device__ __forceinline__ void add_not_finite(const char* vs, int kb, uint32_t sees, f32x16_t (&o)[kO]) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            bf16x8_t ones;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ones[e] = (__bf16)((sees >> (8 * u + e)) & 1 ? 1.f : 0.f);
+#pragma unroll
+            for (int t = 0; t < kO; ++t) {
+                const u32x4_t x = __builtin_bit_cast(u32x4_t, v_operand(vs, kb, u, t));
+#pragma unroll 1
+                for (uint32_t sign = 0; sign < 2; ++sign) {    // the positive infinities and the NaNs, then the negative ones and the NaNs
+                    u32x4_t y;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t lo = x[w] & 0xffffu, up = x[w] >> 16, inf = 0x7f80u | sign << 15;
+                        y[w] = (lo == inf || (lo & 0x7fffu) > 0x7f80u ? 0x3f80u : 0u) | (up == inf || (up & 0x7fffu) > 0x7f80u ? 0x3f800000u : 0u);
+                    }
+                    const f32x16_t n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, y), ones, f32x16_t{}, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[t][r] += n[r] > 0.f ? (sign ? -INFINITY : INFINITY) : 0.f;
+                }
+            }
+        }
+    }
+    __device__ static __forceinline__ u32x4_t finite(u32x4_t x) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) x[w] &= ~not_finite(x[w]);
+        return x;
+    }
+    // dims of registers 4 g .. 4 g + 3 of block t are consecutive
+    __device__ static __forceinline__ void store(float* dst, const f32x16_t (&o)[kO], float f, int lane) {
+#pragma unroll
+        for (int t = 0; t < kO; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4_t*>(dst + 32 * t + 8 * g + 4 * (lane >> 5)) =
+                    f32x4_t{o[t][4 * g] * f, o[t][4 * g + 1] * f, o[t][4 * g + 2] * f, o[t][4 * g + 3] * f};
+    }
+    __device__ static __forceinline__ void store(bf16_t* dst, const f32x16_t (&o)[kO], float f, int lane) {
+#pragma unroll
+        for (int t = 0; t < kO; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                u32x2_t x;
+                x[0] = (uint32_t)f32_to_bf16(o[t][4 * g] * f) | ((uint32_t)f32_to_bf16(o[t][4 * g + 1] * f) << 16);
+                x[1] = (uint32_t)f32_to_bf16(o[t][4 * g + 2] * f) | ((uint32_t)f32_to_bf16(o[t][4 * g + 3] * f) << 16);
+                *reinterpret_cast<u32x2_t*>(dst + 32 * t + 8 * g + 4 * (lane >> 5)) = x;
+            }
+    }
+};
+
+template <int D>
+struct Tile32<float, D> {
+    static constexpr int kKeys = 32, kRow = 4 * D, kO = D / 32;
+    f32x4_t q[D / 8];                                      // dims 8 i + 4 hi .. + 3
+    int k_off, v_off;
+
+    __device__ static __forceinline__ int swizzle(int row) { return row & 15; }
+    __device__ __forceinline__ void init(int lane) {
+        const int c = lane & 31, hi = lane >> 5;
+        k_off = c * kRow + ((hi ^ swizzle(c)) << 4);       // piece 2 i + hi of row c: ^ (i << 5)
+        v_off = 4 * hi * kRow + ((c * kO * 4) ^ (hi << 6)); // dims kO c .. of value row 4 hi, whose pieces are XORed with the key
+    }
+    __device__ __forceinline__ void fresh_offsets() { asm volatile("" : "+v"(k_off), "+v"(v_off)); }
+    __device__ __forceinline__ void load_q(const float* row, bool live, int lane) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            q[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (live) q[i] = *reinterpret_cast<const f32x4_t*>(row + 8 * i + 4 * (lane >> 5));
+        }
+    }
+    __device__ __forceinline__ f32x16_t scores(const char* ks, int) const {
+        f32x16_t s = {};
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            const f32x4_t k = *reinterpret_cast<const f32x4_t*>(ks + (k_off ^ (i << 5)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[i][e], s, 0, 0, 0);
+        }
+        return s;
+    }
+    using piece_t = typename std::conditional<D == 128, f32x4_t, __attribute__((ext_vector_type(2))) float>::type;
+    __device__ __forceinline__ piece_t v_operand(const char* vs, int r) const {      // key 8 (r / 4) + 4 hi + r % 4
+        return *reinterpret_cast<const piece_t*>(vs + (8 * (r >> 2) + (r & 3)) * kRow + (v_off ^ ((8 * (r >> 2 & 1) + (r & 3)) << 4)));
+    }
+    __device__ __forceinline__ void weigh(const char* vs, int, const f32x16_t& p, f32x16_t (&o)[kO]) const {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const piece_t v = v_operand(vs, r);
+#pragma unroll
+            for (int c = 0; c < kO; ++c) o[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[c], p[r], o[c], 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void add_not_finite(const char* vs, int, uint32_t sees, f32x16_t (&o)[kO]) const {
+#pragma unroll
+        for (int c = 0; c < kO; ++c) {
+#pragma unroll 1
+            for (int sign = 0; sign < 2; ++sign) {
+                f32x16_t n = {};
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float v = v_operand(vs, r)[c];
+                    const bool bad = not_finite(v) && !(sign ? v > 0.f : v < 0.f);
+                    n = __builtin_amdgcn_mfma_f32_32x32x2f32(bad ? 1.f : 0.f, (sees >> r) & 1 ? 1.f : 0.f, n, 0, 0, 0);
+                }
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[c][x] += n[x] > 0.f ? (sign ? -INFINITY : INFINITY) : 0.f;
+            }
+        }
+    }
+    __device__ static __forceinline__ u32x4_t finite(u32x4_t x) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) x[w] = not_finite(__uint_as_float(x[w])) ? 0u : x[w];
+        return x;
+    }
+    // register r of block c is dim kO (8 (r / 4) + 4 hi + r % 4) + c
+    __device__ static __forceinline__ void store(float* dst, const f32x16_t (&o)[kO], float f, int lane) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int c = 0; c < kO; ++c) dst[kO * (8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) + c] = o[c][r] * f;
+    }
+};
+
+// Many rows for each list of keys (prompts; all rows of a group against its prefix): a tile of 128 (row, head of the group)
+// pairs of one key head against one part of a list; wave w has pairs 32 w .., and the four share the keys and values that
+// LDS-DMA brings one tile ahead.  Bound by the matrix instructions.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls, int tiles) {
+    using Tile = Tile32<T, D>;
+    constexpr int KT = Tile::kKeys, ROW = Tile::kRow, PIECES = ROW / 16, GROUPS = KT / 16;
+    constexpr int RPI = 1024 / ROW, NI = KT / 4 / RPI;     // rows of one DMA instruction, instructions of a wave for a tile
+    __shared__ __attribute__((aligned(1024))) char smem[2][2][KT * ROW];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int G = a.hq / a.hk;
+    int bid = blockIdx.x;
+    const int hk = bid % a.hk;                             // workgroups of one key head meet in the same L2 (8 XCDs, dealt in turn)
+    bid /= a.hk;
+    const int split = bid % ls.splits;
+    // Tiles are numbered so that list i has those from floor(r0 G / 128) + i on, which leaves every list as many as it needs.
+    // Late tiles first: under a causal mask they have the most keys.
+    const int tile = tiles - 1 - bid / ls.splits;
+    int list = 0;
+    {
+        int c = 0;
+        for (int i = lane; i < ls.n; i += 64) {
+            int s1 = i + 1;
+            if (ls.group_starts) s1 = min(max(ls.group_starts[i + 1], 0), a.n_seqs);
+            int r1 = a.q_starts ? a.q_starts[s1] : s1;
+            r1 = min(max(r1, 0), a.rows);
+            c += (int)((int64_t)r1 * G >> 7) + i + 1 <= tile ? 1 : 0;
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) c += __shfl_xor(c, off, 64);
+        list = __builtin_amdgcn_readfirstlane(c);
+    }
+    if (list >= ls.n) return;
+    int r0, r1, keys, k0, k1;
+    list_extent(a, ls, list, r0, r1, keys);
+    part_range(keys, ls.splits, split, k0, k1);
+    const int n_rows = (r1 - r0) * G;
+    const int t0 = (tile - (int)((int64_t)r0 * G >> 7) - list) * 128;
+    if (t0 < 0 || t0 >= n_rows) return;
+
+    const int mine = t0 + 32 * wave + (lane & 31);
+    const bool live = mine < n_rows;
+    const int row = r0 + (live ? mine / G : 0);
+    const int head = hk * G + (live ? mine % G : 0);
+    const int at_end = keys - (r1 - r0) + 1;               // keys that the list's first row sees
+    const int limit = ls.causal ? keys - (r1 - row) + 1 : keys;
+    const int tile_end = min(k1, ls.causal ? at_end + min(t0 + 127, n_rows - 1) / G : keys);
+    const int tile_first = ls.causal ? at_end + t0 / G : keys;
+    const bool wave_live = t0 + 32 * wave < n_rows;
+    const int wave_first = ls.causal ? at_end + (t0 + 32 * wave) / G : keys;
+    const int wave_end = !wave_live ? 0 : min(k1, ls.causal ? at_end + min(t0 + 32 * wave + 31, n_rows - 1) / G : keys);
+
+    Tile t;
+    t.init(lane);
+    t.load_q(reinterpret_cast<const T*>(a.q) + (int64_t)row * a.q_row + (int64_t)head * a.q_head, live, lane);
+    f32x16_t o[Tile::kO];
+#pragma unroll
+    for (int c = 0; c < Tile::kO; ++c) o[c] = f32x16_t{};
+    float m = -INFINITY, l = 0.f;
+    bool seen = false;
+
+    // pages of the 16-key groups of a tile
+    auto pages_of = [&](int kt, int (&ids)[GROUPS]) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) ids[g] = kt + 16 * g < tile_end ? ls.table.page(list, kt + 16 * g) : -1;
+    };
+    // wave w brings rows w KT / 4 .. of a tile, which lie in one page; the rows of a page that is not there come from page 0
+    auto request = [&](int kt, const int (&ids)[GROUPS], int buf) {
+        const int first = wave * (KT / 4), id = ids[first / 16];
+        const int at_group = id < 0 ? 0 : (kt + (first & ~15)) & ((1 << ls.table.page_shift) - 1);
+        const size_t base = ((((size_t)max(id, 0) * a.hk + hk) << ls.table.page_shift) + at_group) * ROW;
+        const char* kbase = reinterpret_cast<const char*>(a.kp) + base;
+        const char* vbase = reinterpret_cast<const char*>(a.vp) + base;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            const int r = first + j * RPI + lane / PIECES;
+            const uint32_t off = (r & 15) * ROW + (((lane % PIECES) ^ Tile::swizzle(r)) << 4);
+            __builtin_amdgcn_global_load_lds((gptr_t)(kbase + off), (lptr_t)(&smem[buf][0][(first + j * RPI) * ROW]), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr_t)(vbase + off), (lptr_t)(&smem[buf][1][(first + j * RPI) * ROW]), 16, 0, 0);
+        }
+    };
+    int ids[GROUPS], ids_next[GROUPS];
+    pages_of(k0, ids);
+    if (k0 < tile_end) request(k0, ids, 0);
+    pages_of(k0 + KT, ids_next);
+    int buf = 0;
+    for (int kt = k0; kt < tile_end; kt += KT) {
+        __syncthreads();                                   // this tile has landed, and every wave is done with the other buffer
+        const char* ks = smem[buf][0];
+        char* vs = smem[buf][1];
+        uint32_t absent = 0;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) absent |= ids[g] < 0 ? 1u << g : 0u;
+        // Some keys are not there, or some rows of the workgroup do not see all of them: look for values that are not finite,
+        // whose product with a weight of 0 would not be 0.
+        bool apart = false;
+        if (absent != 0 || kt + KT > min(tile_first, tile_end)) {
+#pragma unroll 1
+            for (int i = threadIdx.x * 16; i < KT * ROW; i += 4096) {
+                const u32x4_t x = *reinterpret_cast<const u32x4_t*>(vs + i), y = Tile::finite(x);
+                apart |= x[0] != y[0] || x[1] != y[1] || x[2] != y[2] || x[3] != y[3];
+            }
+            apart = __syncthreads_or(apart);
+        }
+        if (kt + KT < tile_end) request(kt + KT, ids_next, buf ^ 1);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) ids[g] = ids_next[g];
+        pages_of(kt + 2 * KT, ids_next);
+
+        const bool active = kt < wave_end;
+        f32x16_t s[KT / 32];
+        uint32_t sees[KT / 32];
+        if (active) {
+            t.fresh_offsets();
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) s[kb] = t.scores(ks, kb);
+            if (absent != 0 || kt + KT > min(wave_first, tile_end)) {
+#pragma unroll
+                for (int kb = 0; kb < KT / 32; ++kb) {
+                    sees[kb] = 0;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = 32 * kb + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                        const bool vis = kt + i < limit && kt + i < tile_end && !(absent >> (i >> 4) & 1);
+                        if (!vis) s[kb][r] = -INFINITY;
+                        sees[kb] |= vis ? 1u << r : 0u;
+                    }
+                    seen |= sees[kb] != 0;
+                }
+            } else {
+                seen = true;
+#pragma unroll
+                for (int kb = 0; kb < KT / 32; ++kb) sees[kb] = 0xffffu;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (__any(top > m)) {                          // else the running maxima stand and nothing is scaled
+                const float mn = fmaxf(m, top);
+                const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+                m = mn;
+                l *= w;
+#pragma unroll
+                for (int c = 0; c < Tile::kO; ++c) o[c] *= w;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[kb][r] = __builtin_amdgcn_exp2f((s[kb][r] - ref) * a.scale_log2);
+                    l += s[kb][r];
+                }
+            }
+        }
+        if (__builtin_expect(apart, 0)) {
+            if (active) {
+#pragma unroll
+                for (int kb = 0; kb < KT / 32; ++kb) t.add_not_finite(vs, kb, sees[kb], o);
+            }
+            __syncthreads();
+#pragma unroll 1
+            for (int i = threadIdx.x * 16; i < KT * ROW; i += 4096)
+                *reinterpret_cast<u32x4_t*>(vs + i) = Tile::finite(*reinterpret_cast<const u32x4_t*>(vs + i));
+            __syncthreads();
+        }
+        if (active) {
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) t.weigh(vs, kb, s[kb], o);
+        }
+        buf ^= 1;
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    int any = seen ? 1 : 0;
+    any |= __shfl_xor(any, 32, 64);
+    if (any && m == -INFINITY) m = -FLT_MAX;               // as in k_paged_few
+    if (!live) return;
+    const size_t at = (size_t)row * a.hq + head;
+    if (a.part_o) {
+        const size_t part = (size_t)(ls.part0 + split) * ((size_t)a.rows * a.hq) + at;
+        Tile::store(a.part_o + part * D, o, 1.f, lane);
+        if (lane < 32) a.part_ml[part] = make_float2(m, l);
+    } else {
+        Tile::store(reinterpret_cast<T*>(a.out) + at * D, o, any ? 1.f / l : 0.f, lane);
+    }
+}
+
 struct JoinArgs {
     int parts, prefix_parts;         // the prefix's parts come first
     const int32_t* group_starts;     // null: no prefix
@@ -491,34 +884,44 @@ static int check_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     return LCMHIP_OK;
 }
 
-// How a call is cut: parts of the own keys and of the prefix.  One workgroup walks one part for one key head and 16 rows; parts
-// are added until the grid has kWanted workgroups, and none is shorter than kMinPart.
-constexpr int kWanted = 2048, kMaxParts = 64;
+// How a call is cut.  A list of keys goes to k_paged_few where its rows fill no more than one tile of 16, else to k_paged_many.
+// Parts are added until the grid has kWanted workgroups, and none is shorter than kMinPart.
+constexpr int kWantedFew = 2048, kWantedMany = 512, kMaxParts = 64;
+struct ListPlan {
+    bool many = false;
+    int tiles = 1;             // few: tiles a list, many: tiles in all
+    int splits = 0;
+};
 struct Plan {
-    int own_splits = 1, prefix_splits = 0, own_tiles = 1, prefix_tiles = 1;
+    ListPlan own, prefix;
     bool joined = false;
-    int64_t part_rows = 0;
     size_t ml_bytes = 0, bytes = 0;
 };
 
-static int splits_for(int64_t blocks, int max_keys) {
+static ListPlan plan_lists(int64_t lists, int64_t list_rows, int64_t all_rows, int hk, int max_keys) {
+    ListPlan p;
+    p.many = list_rows > 16;
+    int64_t blocks = lists * hk;
+    if (p.many) {
+        p.tiles = (int)(all_rows / 128 + lists);
+        blocks = (all_rows + 127) / 128 * hk;
+    }
+    const int64_t wanted = (p.many ? kWantedMany : kWantedFew) / std::max<int64_t>(blocks, 1);
     const int64_t most = std::min<int64_t>(kMaxParts, (max_keys + kMinPart - 1) / kMinPart);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(most, kWanted / std::max<int64_t>(blocks, 1)));
+    p.splits = (int)std::max<int64_t>(1, std::min(most, wanted));
+    return p;
 }
 
 static Plan make_plan(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, const lcmhip_shared_prefix* prefix, int64_t rows,
                       int n_heads) {
     Plan p;
-    const int G = n_heads / pages->n_kv_heads;
-    p.own_tiles = (int)std::min<int64_t>(((int64_t)batch->max_q * G + 15) / 16, (rows * G + 15) / 16);
-    p.own_splits = splits_for((int64_t)batch->n_seqs * pages->n_kv_heads * p.own_tiles, batch->max_keys);
-    if (prefix) {
-        p.prefix_tiles = (int)((rows * G + 15) / 16);
-        p.prefix_splits = splits_for((int64_t)pages->n_kv_heads * (p.prefix_tiles + prefix->n_groups), prefix->max_keys);
-    }
-    p.joined = p.own_splits + p.prefix_splits > 1;
+    const int64_t G = n_heads / pages->n_kv_heads;
+    p.own = plan_lists(batch->n_seqs, std::min<int64_t>(batch->max_q, rows) * G, rows * G, pages->n_kv_heads, batch->max_keys);
+    if (prefix)
+        p.prefix = plan_lists(prefix->n_groups, (rows + prefix->n_groups - 1) / prefix->n_groups * G, rows * G, pages->n_kv_heads, prefix->max_keys);
+    p.joined = p.own.splits + p.prefix.splits > 1;
     if (p.joined) {
-        const size_t n = (size_t)(p.own_splits + p.prefix_splits) * rows * n_heads;
+        const size_t n = (size_t)(p.own.splits + p.prefix.splits) * rows * n_heads;
         p.ml_bytes = (n * sizeof(float2) + 255) & ~(size_t)255;
         p.bytes = p.ml_bytes + n * pages->head_dim * sizeof(float);
     }
@@ -527,19 +930,20 @@ static Plan make_plan(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* ba
 
 template <typename T, int D>
 static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists& prefix, const Plan& p, hipStream_t st) {
-    auto few = [&](const KeyLists& ls, int tiles) {
-        const int64_t blocks = (int64_t)a.hk * ls.splits * ls.n * tiles;
+    auto attend = [&](const KeyLists& ls, const ListPlan& lp) {
+        const int64_t blocks = (int64_t)a.hk * ls.splits * (lp.many ? lp.tiles : (int64_t)ls.n * lp.tiles);
         LCM_REQUIRE(blocks <= INT32_MAX, "paged attention: too many rows");
-        hipLaunchKernelGGL((k_paged_few<T, D>), dim3((unsigned)blocks), dim3(256), 0, st, a, ls, tiles);
+        if (lp.many) hipLaunchKernelGGL((k_paged_many<T, D>), dim3((unsigned)blocks), dim3(256), 0, st, a, ls, lp.tiles);
+        else hipLaunchKernelGGL((k_paged_few<T, D>), dim3((unsigned)blocks), dim3(256), 0, st, a, ls, lp.tiles);
         LCM_HIP_CHECK(hipGetLastError());
         return LCMHIP_OK;
     };
-    if (prefix.n > 0) LCM_TRY(few(prefix, p.prefix_tiles));
-    LCM_TRY(few(own, p.own_tiles));
+    if (prefix.n > 0) LCM_TRY(attend(prefix, p.prefix));
+    LCM_TRY(attend(own, p.own));
     if (p.joined) {
         const int64_t per = 256 / (D / 4);
         hipLaunchKernelGGL((k_paged_join<T, D>), dim3((unsigned)(((int64_t)a.rows * a.hq + per - 1) / per)), dim3(256), 0, st, a,
-                           JoinArgs{p.own_splits + p.prefix_splits, p.prefix_splits, prefix.group_starts, prefix.n});
+                           JoinArgs{p.own.splits + p.prefix.splits, p.prefix.splits, prefix.group_starts, prefix.n});
         LCM_HIP_CHECK(hipGetLastError());
     }
     return LCMHIP_OK;
@@ -563,12 +967,12 @@ static int paged_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     a.q_starts = batch->q_starts; a.n_seqs = batch->n_seqs;
     a.rows = (int)rows; a.hq = n_heads; a.hk = pages->n_kv_heads;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const KeyLists own{PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), pages->n_pages}, batch->seq_lens, nullptr,
-                     batch->n_seqs, batch->max_keys, causal != 0, p.own_splits, p.prefix_splits};
+    const KeyLists own{PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), (uint32_t)pages->n_pages}, batch->seq_lens, nullptr,
+                     batch->n_seqs, batch->max_keys, causal != 0, p.own.splits, p.prefix.splits};
     KeyLists pre{};
     if (prefix)
-        pre = KeyLists{PageTable{prefix->page_table, prefix->max_pages, page_shift_of(pages), pages->n_pages}, prefix->lens,
-                            prefix->group_starts, prefix->n_groups, prefix->max_keys, 0, p.prefix_splits, 0};
+        pre = KeyLists{PageTable{prefix->page_table, prefix->max_pages, page_shift_of(pages), (uint32_t)pages->n_pages}, prefix->lens,
+                            prefix->group_starts, prefix->n_groups, prefix->max_keys, 0, p.prefix.splits, 0};
     if (p.joined) {
         a.part_ml = reinterpret_cast<float2*>(ws);
         a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + p.ml_bytes);

@@ -269,7 +269,7 @@ int lcmhip_paged_append(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* 
     a.rows = rows; a.nq = q ? n_heads : 0; a.nk = a.nv = pages->n_kv_heads;
     a.positions = positions;
     a.k_pages = pages->k; a.v_pages = pages->v;
-    a.table = PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), pages->n_pages};
+    a.table = PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), (uint32_t)pages->n_pages};
     a.seq_lens = batch->seq_lens; a.q_starts = batch->q_starts; a.n_seqs = batch->n_seqs; a.max_keys = batch->max_keys;
     return launch_head_rows(a, pages->head_dim, pages->dtype, true, static_cast<hipStream_t>(stream));
 }
