@@ -55,11 +55,12 @@ __device__ __forceinline__ void list_extent(const PagedArgs& a, const KeyLists& 
     keys = max(0, min(read_index(ls.lens + i), ls.max_keys));
 }
 
-// Part `split` of `keys` keys: at most `splits` equal parts, multiples of 32 keys, of no fewer than kMinPart.
-constexpr int kMinPart = 256;
-__device__ __forceinline__ void part_range(int keys, int splits, int split, int& k0, int& k1) {
-    const int n = max(1, min(splits, (keys + kMinPart - 1) / kMinPart));
-    const int len = ((keys + n - 1) / n + 31) & ~31;
+constexpr int kMinPartFew = 256;   // keys a workgroup of k_paged_few is worth
+// Part `split` of `keys` keys: at most `splits` equal parts, multiples of STEP keys, of no fewer than `least`.
+template <int STEP>
+__device__ __forceinline__ void part_range(int keys, int splits, int least, int split, int& k0, int& k1) {
+    const int n = max(1, min(splits, (keys + least - 1) / least));
+    const int len = ((keys + n - 1) / n + STEP - 1) / STEP * STEP;
     k0 = min(keys, split * len);
     k1 = min(keys, k0 + len);
 }
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedArgs a, KeyLists ls, 
     const int G = a.hq / a.hk;
     int r0, r1, keys, k0, k1;
     list_extent(a, ls, list, r0, r1, keys);
-    part_range(keys, ls.splits, split, k0, k1);
+    part_range<32>(keys, ls.splits, kMinPartFew, split, k0, k1);
     const int n_rows = (r1 - r0) * G;
     const T* kp = reinterpret_cast<const T*>(a.kp);
     const T* vp = reinterpret_cast<const T*>(a.vp);
@@ -656,7 +657,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
     if (list >= ls.n) return;
     int r0, r1, keys, k0, k1;
     list_extent(a, ls, list, r0, r1, keys);
-    part_range(keys, ls.splits, split, k0, k1);
+    part_range<KT>(keys, ls.splits, 2 * KT, split, k0, k1);
     const int n_rows = (r1 - r0) * G;
     const int t0 = (tile - (int)((int64_t)r0 * G >> 7) - list) * 128;
     if (t0 < 0 || t0 >= n_rows) return;
@@ -818,51 +819,78 @@ struct JoinArgs {
     int n_groups;
 };
 
-// Joins the parts of every (row, head): D / 4 lanes each, which hold the statistics of the parts between them.
-template <typename T, int D>
+// Joins the parts of every (row, head).  D / 4 lanes hold a row's values; PG such groups take the parts in turn and meet in LDS
+// (many parts of few rows), or one group takes them all (PG = 1).
+template <typename T, int D, int PG>
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, JoinArgs j) {
-    constexpr int L4 = D / 4;
-    const int64_t at = (int64_t)blockIdx.x * (256 / L4) + threadIdx.x / L4;
-    const int sub = threadIdx.x % L4;
+    constexpr int L4 = D / 4, ROWS = 256 / L4 / PG, U = 8;
+    __shared__ f32x4_t red_o[PG > 1 ? 256 : 1];
+    __shared__ float2 red_ml[PG > 1 ? 256 / L4 : 1];
+    const int sub = threadIdx.x % L4, group = threadIdx.x / L4, pg = group % PG;
+    const int64_t at = (int64_t)blockIdx.x * ROWS + group / PG;
     const int64_t row = at / a.hq;
     // rows of no sequence are left alone; those of no group have no prefix
-    const int first = a.q_starts ? a.q_starts[0] : 0, last = a.q_starts ? a.q_starts[a.n_seqs] : a.n_seqs;
+    const int first = a.q_starts ? read_index(a.q_starts) : 0, last = a.q_starts ? read_index(a.q_starts + a.n_seqs) : a.n_seqs;
     const bool live = row < a.rows && row >= first && row < last;
     int part0 = j.prefix_parts;
     if (j.group_starts) {
-        const int s0 = min(max(j.group_starts[0], 0), a.n_seqs), s1 = min(max(j.group_starts[j.n_groups], 0), a.n_seqs);
-        if (row >= (a.q_starts ? a.q_starts[s0] : s0) && row < (a.q_starts ? a.q_starts[s1] : s1)) part0 = 0;
+        const int s0 = min(max(read_index(j.group_starts), 0), a.n_seqs), s1 = min(max(read_index(j.group_starts + j.n_groups), 0), a.n_seqs);
+        if (row >= (a.q_starts ? read_index(a.q_starts + s0) : s0) && row < (a.q_starts ? read_index(a.q_starts + s1) : s1)) part0 = 0;
     }
     const int64_t stride = (int64_t)a.rows * a.hq;
-    float M = -INFINITY;
-    for (int p = part0 + sub; p < j.parts; p += L4)
-        if (live) M = fmaxf(M, a.part_ml[p * stride + at].x);
-#pragma unroll
-    for (int off = L4 / 2; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
-    float L = 0.f;
+    float m = -INFINITY, l = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = part0; p0 < j.parts; p0 += L4) {
-        const int p = p0 + sub;
-        float w = 0.f;
-        if (live && p < j.parts) {
-            const float2 ml = a.part_ml[p * stride + at];
-            if (ml.x != -INFINITY) {
-                w = __builtin_amdgcn_exp2f((ml.x - M) * a.scale_log2);
-                L += ml.y * w;
-            }
-        }
-        const int n = min(L4, j.parts - p0);
-        for (int i = 0; i < n; ++i) {
-            const float f = __shfl(w, i, L4);
-            if (f > 0.f) acc += *reinterpret_cast<const f32x4_t*>(a.part_o + ((p0 + i) * stride + at) * D + 4 * sub) * f;
-        }
-    }
+    // U parts at a time: all their loads are in flight before the first is used
+    for (int p0 = live ? part0 + pg : j.parts; p0 < j.parts; p0 += U * PG) {
+        float2 ml[U];
+        f32x4_t o[U];
 #pragma unroll
-    for (int off = L4 / 2; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
+        for (int u = 0; u < U; ++u) {
+            const int64_t x = min(p0 + u * PG, j.parts - 1) * stride + at;
+            ml[u] = a.part_ml[x];
+            o[u] = *reinterpret_cast<const f32x4_t*>(a.part_o + x * D + 4 * sub);
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (p0 + u * PG >= j.parts) ml[u].x = -INFINITY;
+            mn = fmaxf(mn, ml[u].x);
+        }
+        const float w0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+        l *= w0;
+        acc *= w0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (ml[u].x == -INFINITY) continue;            // an empty part wrote no values
+            const float w = __builtin_amdgcn_exp2f((ml[u].x - mn) * a.scale_log2);
+            l += ml[u].y * w;
+            acc += o[u] * w;
+        }
+        m = mn;
+    }
+    if (PG > 1) {
+        red_o[threadIdx.x] = acc;
+        if (sub == 0) red_ml[group] = make_float2(m, l);
+        __syncthreads();
+        if (pg != 0) return;
+        float M = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < PG; ++g) M = fmaxf(M, red_ml[group + g].x);
+        l = 0.f;
+        acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < PG; ++g) {
+            const float2 ml = red_ml[group + g];
+            const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * a.scale_log2);
+            l += ml.y * w;
+            acc += red_o[threadIdx.x + g * L4] * w;
+        }
+        m = M;
+    }
     if (live) {
         T* dst = reinterpret_cast<T*>(a.out) + at * D + 4 * sub;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) Elem<T>::store(dst + e, M == -INFINITY ? 0.f : acc[e] / L);
+        for (int e = 0; e < 4; ++e) Elem<T>::store(dst + e, m == -INFINITY ? 0.f : acc[e] / l);
     }
 }
 
@@ -885,8 +913,11 @@ static int check_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
 }
 
 // How a call is cut.  A list of keys goes to k_paged_few where its rows fill no more than one tile of 16, else to k_paged_many.
-// Parts are added until the grid has kWanted workgroups, and none is shorter than kMinPart.
-constexpr int kWantedFew = 2048, kWantedMany = 512, kMaxParts = 64;
+// few: parts are added until the grid has kWantedFew workgroups, four for each place on the chip, so that lists of unequal
+//      length even out.
+// many: a part takes a workgroup a step for each tile of keys and a few to begin and end, a round of kPlaces workgroups at a
+//      time, and its rows' partial results are written and read once; the number of parts that makes the sum least.
+constexpr int kWantedFew = 2048, kPlaces = 512, kMaxParts = 64;
 struct ListPlan {
     bool many = false;
     int tiles = 1;             // few: tiles a list, many: tiles in all
@@ -898,17 +929,30 @@ struct Plan {
     size_t ml_bytes = 0, bytes = 0;
 };
 
-static ListPlan plan_lists(int64_t lists, int64_t list_rows, int64_t all_rows, int hk, int max_keys) {
+static ListPlan plan_lists(int64_t lists, int64_t list_rows, int64_t all_rows, int hk, int max_keys, int head_dim, int dtype) {
     ListPlan p;
     p.many = list_rows > 16;
-    int64_t blocks = lists * hk;
-    if (p.many) {
-        p.tiles = (int)(all_rows / 128 + lists);
-        blocks = (all_rows + 127) / 128 * hk;
+    if (!p.many) {
+        const int64_t most = std::min<int64_t>(kMaxParts, (max_keys + kMinPartFew - 1) / kMinPartFew);
+        p.splits = (int)std::max<int64_t>(1, std::min(most, kWantedFew / std::max<int64_t>(lists * hk, 1)));
+        return p;
     }
-    const int64_t wanted = (p.many ? kWantedMany : kWantedFew) / std::max<int64_t>(blocks, 1);
-    const int64_t most = std::min<int64_t>(kMaxParts, (max_keys + kMinPart - 1) / kMinPart);
-    p.splits = (int)std::max<int64_t>(1, std::min(most, wanted));
+    p.tiles = (int)(all_rows / 128 + lists);
+    // workgroups of one part, if the lists have about as many rows each
+    const int64_t blocks = hk * std::max((all_rows + 127) / 128, lists * ((all_rows / lists + 127) / 128));
+    const int step_keys = dtype == LCMHIP_BF16 ? 64 : 32;
+    const double step_us = (dtype == LCMHIP_BF16 ? 0.9 : 6.8) * head_dim / 128;
+    const double join_us = (double)all_rows * hk * head_dim * 8 / 3e6;
+    const int most = std::min(kMaxParts, (max_keys + 2 * step_keys - 1) / (2 * step_keys));
+    double best = 0;
+    for (int s = 1; s <= most; ++s) {
+        const int64_t rounds = (blocks * s + kPlaces - 1) / kPlaces, steps = (max_keys + (int64_t)s * step_keys - 1) / ((int64_t)s * step_keys);
+        const double cost = (double)rounds * (steps * step_us + 3.0) + (s > 1 ? 4.0 + s * join_us : 0.0);
+        if (s == 1 || cost < best) {
+            best = cost;
+            p.splits = s;
+        }
+    }
     return p;
 }
 
@@ -916,9 +960,10 @@ static Plan make_plan(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* ba
                       int n_heads) {
     Plan p;
     const int64_t G = n_heads / pages->n_kv_heads;
-    p.own = plan_lists(batch->n_seqs, std::min<int64_t>(batch->max_q, rows) * G, rows * G, pages->n_kv_heads, batch->max_keys);
+    if (batch->n_seqs == 0 || rows == 0) return p;
+    p.own = plan_lists(batch->n_seqs, std::min<int64_t>(batch->max_q, rows) * G, rows * G, pages->n_kv_heads, batch->max_keys, pages->head_dim, pages->dtype);
     if (prefix)
-        p.prefix = plan_lists(prefix->n_groups, (rows + prefix->n_groups - 1) / prefix->n_groups * G, rows * G, pages->n_kv_heads, prefix->max_keys);
+        p.prefix = plan_lists(prefix->n_groups, (rows + prefix->n_groups - 1) / prefix->n_groups * G, rows * G, pages->n_kv_heads, prefix->max_keys, pages->head_dim, pages->dtype);
     p.joined = p.own.splits + p.prefix.splits > 1;
     if (p.joined) {
         const size_t n = (size_t)(p.own.splits + p.prefix.splits) * rows * n_heads;
@@ -941,9 +986,13 @@ static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists&
     if (prefix.n > 0) LCM_TRY(attend(prefix, p.prefix));
     LCM_TRY(attend(own, p.own));
     if (p.joined) {
-        const int64_t per = 256 / (D / 4);
-        hipLaunchKernelGGL((k_paged_join<T, D>), dim3((unsigned)(((int64_t)a.rows * a.hq + per - 1) / per)), dim3(256), 0, st, a,
-                           JoinArgs{p.own.splits + p.prefix.splits, p.prefix.splits, prefix.group_starts, prefix.n});
+        // one group of lanes for a row while the rows alone fill the chip, else eight
+        const JoinArgs j{p.own.splits + p.prefix.splits, p.prefix.splits, prefix.group_starts, prefix.n};
+        const int64_t heads = (int64_t)a.rows * a.hq, per = 256 / (D / 4);
+        if (heads / per >= 1024 || j.parts <= 8)
+            hipLaunchKernelGGL((k_paged_join<T, D, 1>), dim3((unsigned)((heads + per - 1) / per)), dim3(256), 0, st, a, j);
+        else
+            hipLaunchKernelGGL((k_paged_join<T, D, 8>), dim3((unsigned)((heads + per / 8 - 1) / (per / 8))), dim3(256), 0, st, a, j);
         LCM_HIP_CHECK(hipGetLastError());
     }
     return LCMHIP_OK;

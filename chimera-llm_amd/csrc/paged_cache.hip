@@ -28,8 +28,16 @@ struct HeadArgs {
     int n_seqs, max_keys;
 };
 
+// Eight values as they lie in memory.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<bf16_t> { uint4 x; };
+template <>
+struct Raw8<float> { float4 x, y; };
+
 // HPT heads for each lane group; SLOTS * HPT consecutive heads (query heads, key heads, value heads of row 0, of row 1, ..)
-// for each workgroup.
+// for each workgroup.  All loads of a lane group's heads are in flight before the first is worked on.
 template <typename T, int D, bool APPEND, int HPT>
 __global__ __launch_bounds__(256) void k_head_rows(HeadArgs a) {
     constexpr int LPH = D / 8, SLOTS = 256 / LPH;
@@ -41,6 +49,9 @@ __global__ __launch_bounds__(256) void k_head_rows(HeadArgs a) {
     int seq0 = 0;
     if (APPEND && a.q_starts) seq0 = wave_count_le(a.q_starts + 1, a.n_seqs, row0);
 
+    Raw8<T> raw[HPT];
+    T* dst[HPT];
+    int kinds[HPT], poss[HPT];
 #pragma unroll
     for (int it = 0; it < HPT; ++it) {
         const unsigned u = (unsigned)rem0 + slot + it * SLOTS;
@@ -50,8 +61,13 @@ __global__ __launch_bounds__(256) void k_head_rows(HeadArgs a) {
         const int kind = h < a.nq ? 0 : (h < a.nq + a.nk ? 1 : 2);
         if (kind >= 1) h -= a.nq;
         if (kind == 2) h -= a.nk;
+        const T* src = kind == 0 ? reinterpret_cast<const T*>(a.q) + row * a.q_row + h * a.q_head
+                                 : (kind == 1 ? reinterpret_cast<const T*>(a.k) + row * a.k_row + h * a.k_head
+                                              : reinterpret_cast<const T*>(a.v) + row * a.v_row + h * a.v_head);
+        raw[it] = Raw8<T>{};
+        if (live) raw[it] = *reinterpret_cast<const Raw8<T>*>(src + i0);
         int pos = 0;
-        T* dst = nullptr;
+        T* to = nullptr;
         if (APPEND) {
             int c = -1, seq = seq0;
             if (live) {
@@ -74,93 +90,96 @@ __global__ __launch_bounds__(256) void k_head_rows(HeadArgs a) {
                 if (page >= 0) {
                     const int off = c & ((1 << a.table.page_shift) - 1);
                     T* pool = reinterpret_cast<T*>(kind == 1 ? a.k_pages : a.v_pages);
-                    dst = pool + ((((size_t)page * a.nk + h) << a.table.page_shift) + off) * D + i0;
+                    to = pool + ((((size_t)page * a.nk + h) << a.table.page_shift) + off) * D + i0;
                 }
             } else if (live) {
-                dst = reinterpret_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head + i0;
+                to = reinterpret_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head + i0;
             }
         } else if (live) {
             pos = a.positions ? a.positions[row] : 0;
             if (pos >= 0)
-                dst = kind == 0 ? reinterpret_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head + i0
-                                : reinterpret_cast<T*>(a.k_out) + row * a.ko_row + h * a.ko_head + i0;
+                to = kind == 0 ? reinterpret_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head + i0
+                               : reinterpret_cast<T*>(a.k_out) + row * a.ko_row + h * a.ko_head + i0;
         }
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (dst) {
-            const T* src = kind == 0 ? reinterpret_cast<const T*>(a.q) + row * a.q_row + h * a.q_head
-                                     : (kind == 1 ? reinterpret_cast<const T*>(a.k) + row * a.k_row + h * a.k_head
-                                                  : reinterpret_cast<const T*>(a.v) + row * a.v_row + h * a.v_head);
-            load8<T>(src + i0, x);
+        dst[it] = to;
+        kinds[it] = kind;
+        poss[it] = pos;
+    }
+#pragma unroll
+    for (int it = 0; it < HPT; ++it) {
+        if (kinds[it] == 2) {                              // values go as they are
+            if (dst[it]) *reinterpret_cast<Raw8<T>*>(dst[it]) = raw[it];
+            continue;
         }
-        if (kind < 2) {
-            if (a.norm.kind != LCMHIP_NORM_NONE) {
-                if (a.norm.kind != LCMHIP_NORM_RMS) {
-                    float s = 0.f;
+        float x[8];
+        load8<T>(reinterpret_cast<const T*>(&raw[it]), x);
+        if (a.norm.kind != LCMHIP_NORM_NONE) {
+            if (a.norm.kind != LCMHIP_NORM_RMS) {
+                float s = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) s += x[j];
+                for (int j = 0; j < 8; ++j) s += x[j];
 #pragma unroll
-                    for (int off = LPH / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+                for (int off = LPH / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] -= s * (1.f / D);
-                }
-                float s2 = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) s2 += x[j] * x[j];
-#pragma unroll
-                for (int off = LPH / 2; off > 0; off >>= 1) s2 += __shfl_xor(s2, off, 64);
-                const float r = 1.f / sqrtf(s2 * (1.f / D) + a.norm.eps);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= r;
-                const void* w = kind == 0 ? a.norm.q_weight : a.norm.k_weight;
-                const void* b = kind == 0 ? a.norm.q_bias : a.norm.k_bias;
-                if (w) {
-                    float wv[8];
-                    load8<T>(reinterpret_cast<const T*>(w) + i0, wv);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] *= wv[j];
-                }
-                if (b) {
-                    float bv[8];
-                    load8<T>(reinterpret_cast<const T*>(b) + i0, bv);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] += bv[j];
-                }
+                for (int j = 0; j < 8; ++j) x[j] -= s * (1.f / D);
             }
-            if (a.rot.rotary_dim > 0) {
-                const int half = a.rot.rotary_dim >> 1;
-                const bool known = pos < a.rot.n_positions;
-                const size_t trow = (size_t)(known ? max(pos, 0) : 0) * half;
-                if (a.rot.style == LCMHIP_ROTARY_PAIRS) {
-                    if (i0 < a.rot.rotary_dim) {
-                        const float4 cs = *reinterpret_cast<const float4*>(a.rot.cos + trow + i0 / 2);
-                        const float4 sn = *reinterpret_cast<const float4*>(a.rot.sin + trow + i0 / 2);
-                        rope_rotate(x[0], x[1], cs.x, sn.x);
-                        rope_rotate(x[2], x[3], cs.y, sn.y);
-                        rope_rotate(x[4], x[5], cs.z, sn.z);
-                        rope_rotate(x[6], x[7], cs.w, sn.w);
-                    }
-                } else {
-                    const bool first = i0 < half;
-                    const int lane = threadIdx.x & 63;
-                    const int partner = i0 < a.rot.rotary_dim ? lane + (first ? half / 8 : -(half / 8)) : lane;
-                    float y[8];
+            float s2 = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = __shfl(x[j], partner, 64);
-                    if (i0 < a.rot.rotary_dim) {
-                        float cs[8], sn[8];
-                        load8<float>(a.rot.cos + trow + (first ? i0 : i0 - half), cs);
-                        load8<float>(a.rot.sin + trow + (first ? i0 : i0 - half), sn);
+            for (int j = 0; j < 8; ++j) s2 += x[j] * x[j];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = first ? x[j] * cs[j] - y[j] * sn[j] : x[j] * cs[j] + y[j] * sn[j];
-                    }
-                }
-                if (!known) {
+            for (int off = LPH / 2; off > 0; off >>= 1) s2 += __shfl_xor(s2, off, 64);
+            const float r = 1.f / sqrtf(s2 * (1.f / D) + a.norm.eps);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = __builtin_nanf("");
-                }
+            for (int j = 0; j < 8; ++j) x[j] *= r;
+            const void* w = kinds[it] == 0 ? a.norm.q_weight : a.norm.k_weight;
+            const void* b = kinds[it] == 0 ? a.norm.q_bias : a.norm.k_bias;
+            if (w) {
+                float wv[8];
+                load8<T>(reinterpret_cast<const T*>(w) + i0, wv);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= wv[j];
+            }
+            if (b) {
+                float bv[8];
+                load8<T>(reinterpret_cast<const T*>(b) + i0, bv);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] += bv[j];
             }
         }
-        if (dst) store8<T>(dst, x);
+        if (a.rot.rotary_dim > 0) {
+            const int half = a.rot.rotary_dim >> 1, pos = poss[it];
+            const bool known = pos < a.rot.n_positions;
+            const size_t trow = (size_t)(known ? max(pos, 0) : 0) * half;
+            if (a.rot.style == LCMHIP_ROTARY_PAIRS) {
+                if (i0 < a.rot.rotary_dim) {
+                    const float4 cs = *reinterpret_cast<const float4*>(a.rot.cos + trow + i0 / 2);
+                    const float4 sn = *reinterpret_cast<const float4*>(a.rot.sin + trow + i0 / 2);
+                    rope_rotate(x[0], x[1], cs.x, sn.x);
+                    rope_rotate(x[2], x[3], cs.y, sn.y);
+                    rope_rotate(x[4], x[5], cs.z, sn.z);
+                    rope_rotate(x[6], x[7], cs.w, sn.w);
+                }
+            } else {
+                const bool first = i0 < half;
+                const int lane = threadIdx.x & 63;
+                const int partner = i0 < a.rot.rotary_dim ? lane + (first ? half / 8 : -(half / 8)) : lane;
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = __shfl(x[j], partner, 64);
+                if (i0 < a.rot.rotary_dim) {
+                    float cs[8], sn[8];
+                    load8<float>(a.rot.cos + trow + (first ? i0 : i0 - half), cs);
+                    load8<float>(a.rot.sin + trow + (first ? i0 : i0 - half), sn);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = first ? x[j] * cs[j] - y[j] * sn[j] : x[j] * cs[j] + y[j] * sn[j];
+                }
+            }
+            if (!known) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = __builtin_nanf("");
+            }
+        }
+        if (dst[it]) store8<T>(dst[it], x);
     }
 }
 
@@ -169,9 +188,12 @@ static int launch_head_rows_t(const HeadArgs& a, hipStream_t st) {
     constexpr int SLOTS = 256 / (D / 8);
     const int64_t heads = a.rows * (a.nq + a.nk + a.nv);
     if (heads == 0) return LCMHIP_OK;
-    const int64_t blocks = (heads + SLOTS - 1) / SLOTS;
+    // four heads a lane group once that still fills the chip's 256 CUs with eight workgroups each, else one
+    const int hpt = heads >= (int64_t)SLOTS * 4 * 2048 ? 4 : 1;
+    const int64_t blocks = (heads + SLOTS * hpt - 1) / (SLOTS * hpt);
     LCM_REQUIRE(blocks <= INT32_MAX, "head rows: too many rows");
-    hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (hpt == 4) hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     LCM_HIP_CHECK(hipGetLastError());
     return LCMHIP_OK;
 }
