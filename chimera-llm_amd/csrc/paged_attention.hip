@@ -465,14 +465,23 @@ struct Tile32<bf16_t, D> {
             q[st] = __builtin_bit_cast(bf16x8_t, x);
         }
     }
-    __device__ __forceinline__ f32x16_t scores(const char* ks, int kb) const {
+    using kfrag_t = bf16x8_t[D / 16];                      // dims 16 st + 8 hi .. of row lane % 32 of a 32-key block
+    using vfrag_t = bf16x8_t[2 * kO];                      // V^T operands of its two 16-key steps
+    __device__ __forceinline__ void load_k(const char* ks, int kb, kfrag_t& k) const {
+#pragma unroll
+        for (int st = 0; st < D / 16; ++st) k[st] = *reinterpret_cast<const bf16x8_t*>(ks + kb * 32 * kRow + (k_off ^ (st << 5)));
+    }
+    __device__ __forceinline__ f32x16_t scores(const kfrag_t& k) const {
         f32x16_t s = {};
 #pragma unroll
-        for (int st = 0; st < D / 16; ++st) {
-            const bf16x8_t k = *reinterpret_cast<const bf16x8_t*>(ks + kb * 32 * kRow + (k_off ^ (st << 5)));
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[st], s, 0, 0, 0);
-        }
+        for (int st = 0; st < D / 16; ++st) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[st], q[st], s, 0, 0, 0);
         return s;
+    }
+    __device__ __forceinline__ void load_v(const char* vs, int kb, vfrag_t& v) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < kO; ++t) v[u * kO + t] = v_operand(vs, kb, u, t);
     }
     __device__ __forceinline__ bf16x8_t v_operand(const char* vs, int kb, int u, int t) const {
         const char* base = vs + (kb * 32 + u * 16) * kRow;
@@ -487,12 +496,12 @@ struct Tile32<bf16_t, D> {
         for (int e = 0; e < 8; ++e) pf[e] = (__bf16)p[8 * u + e];
         return pf;
     }
-    __device__ __forceinline__ void weigh(const char* vs, int kb, const f32x16_t& p, f32x16_t (&o)[kO]) const {
+    __device__ __forceinline__ void weigh(const vfrag_t& v, const f32x16_t& p, f32x16_t (&o)[kO]) const {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const bf16x8_t pf = p_operand(p, u);
 #pragma unroll
-            for (int t = 0; t < kO; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_operand(vs, kb, u, t), pf, o[t], 0, 0, 0);
+            for (int t = 0; t < kO; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[u * kO + t], pf, o[t], 0, 0, 0);
         }
     }
     // Infinities and NaNs of a block's values for the rows that see them (bit r of `sees`: the key of register r): counted by a
@@ -568,27 +577,33 @@ struct Tile32<float, D> {
             if (live) q[i] = *reinterpret_cast<const f32x4_t*>(row + 8 * i + 4 * (lane >> 5));
         }
     }
-    __device__ __forceinline__ f32x16_t scores(const char* ks, int) const {
+    using kfrag_t = f32x4_t[D / 8];
+    __device__ __forceinline__ void load_k(const char* ks, int, kfrag_t& k) const {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) k[i] = *reinterpret_cast<const f32x4_t*>(ks + (k_off ^ (i << 5)));
+    }
+    __device__ __forceinline__ f32x16_t scores(const kfrag_t& k) const {
         f32x16_t s = {};
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            const f32x4_t k = *reinterpret_cast<const f32x4_t*>(ks + (k_off ^ (i << 5)));
+        for (int i = 0; i < D / 8; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[i][e], s, 0, 0, 0);
-        }
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i][e], q[i][e], s, 0, 0, 0);
         return s;
     }
     using piece_t = typename std::conditional<D == 128, f32x4_t, __attribute__((ext_vector_type(2))) float>::type;
     __device__ __forceinline__ piece_t v_operand(const char* vs, int r) const {      // key 8 (r / 4) + 4 hi + r % 4
         return *reinterpret_cast<const piece_t*>(vs + (8 * (r >> 2) + (r & 3)) * kRow + (v_off ^ ((8 * (r >> 2 & 1) + (r & 3)) << 4)));
     }
-    __device__ __forceinline__ void weigh(const char* vs, int, const f32x16_t& p, f32x16_t (&o)[kO]) const {
+    using vfrag_t = piece_t[16];
+    __device__ __forceinline__ void load_v(const char* vs, int, vfrag_t& v) const {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const piece_t v = v_operand(vs, r);
+        for (int r = 0; r < 16; ++r) v[r] = v_operand(vs, r);
+    }
+    __device__ __forceinline__ void weigh(const vfrag_t& v, const f32x16_t& p, f32x16_t (&o)[kO]) const {
 #pragma unroll
-            for (int c = 0; c < kO; ++c) o[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[c], p[r], o[c], 0, 0, 0);
-        }
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int c = 0; c < kO; ++c) o[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[r][c], p[r], o[c], 0, 0, 0);
     }
     __device__ __forceinline__ void add_not_finite(const char* vs, int, uint32_t sees, f32x16_t (&o)[kO]) const {
 #pragma unroll
@@ -620,6 +635,15 @@ struct Tile32<float, D> {
             for (int c = 0; c < kO; ++c) dst[kO * (8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) + c] = o[c][r] * f;
     }
 };
+
+// 64 lanes bring 16 bytes each, from base + off (base and dst the same for the wave), to dst + 16 lane in LDS.  Written in assembly
+// because the compiler waits for every outstanding LDS-DMA before any LDS read, whatever it reads; nothing is returned in
+// registers, and the waits for the data are the loop's own (s_waitcnt vmcnt before the barrier).  M0 holds nothing across
+// instructions of the compiler.
+__device__ __forceinline__ void lds_dma16(const char* base, uint32_t off, char* dst) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(off), "s"(base) : "memory");
+}
 
 // Many rows for each list of keys (prompts; all rows of a group against its prefix): a tile of 128 (row, head of the group)
 // pairs of one key head against one part of a list; wave w has pairs 32 w .., and the four share the keys and values that
@@ -683,33 +707,46 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
     float m = -INFINITY, l = 0.f;
     bool seen = false;
 
-    // pages of the 16-key groups of a tile
+    // Lane i holds the id of page page0 + i of the list: one load for 64 pages, a lane read for each use.  (Scalar loads inside
+    // the loop would make every wait for an LDS read a wait for all of them.)
+    int page0 = k0 >> ls.table.page_shift, page_ids = ls.table.page(list, (page0 + lane) << ls.table.page_shift);
+    // ids of the 16-key groups of a tile; -1 behind the last key
     auto pages_of = [&](int kt, int (&ids)[GROUPS]) {
+        if (((kt + KT - 1) >> ls.table.page_shift) - page0 >= 64) {
+            page0 = kt >> ls.table.page_shift;
+            page_ids = ls.table.page(list, (page0 + lane) << ls.table.page_shift);
+        }
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) ids[g] = kt + 16 * g < tile_end ? ls.table.page(list, kt + 16 * g) : -1;
+        for (int g = 0; g < GROUPS; ++g)
+            ids[g] = kt + 16 * g < tile_end ? __builtin_amdgcn_readlane(page_ids, ((kt + 16 * g) >> ls.table.page_shift) - page0) : -1;
     };
-    // wave w brings rows w KT / 4 .. of a tile, which lie in one page; the rows of a page that is not there come from page 0
+    // Wave w brings rows w KT / 4 .. of a tile, which lie in one page; the rows of a page that is not there come from page 0.
+    uint32_t dma_off[NI];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+        const int r = wave * (KT / 4) + j * RPI + lane / PIECES;
+        dma_off[j] = (r & 15) * ROW + (((lane % PIECES) ^ Tile::swizzle(r)) << 4);
+    }
     auto request = [&](int kt, const int (&ids)[GROUPS], int buf) {
         const int first = wave * (KT / 4), id = ids[first / 16];
         const int at_group = id < 0 ? 0 : (kt + (first & ~15)) & ((1 << ls.table.page_shift) - 1);
         const size_t base = ((((size_t)max(id, 0) * a.hk + hk) << ls.table.page_shift) + at_group) * ROW;
-        const char* kbase = reinterpret_cast<const char*>(a.kp) + base;
-        const char* vbase = reinterpret_cast<const char*>(a.vp) + base;
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
-            const int r = first + j * RPI + lane / PIECES;
-            const uint32_t off = (r & 15) * ROW + (((lane % PIECES) ^ Tile::swizzle(r)) << 4);
-            __builtin_amdgcn_global_load_lds((gptr_t)(kbase + off), (lptr_t)(&smem[buf][0][(first + j * RPI) * ROW]), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gptr_t)(vbase + off), (lptr_t)(&smem[buf][1][(first + j * RPI) * ROW]), 16, 0, 0);
+            lds_dma16(reinterpret_cast<const char*>(a.kp) + base, dma_off[j], &smem[buf][0][(first + j * RPI) * ROW]);
+            lds_dma16(reinterpret_cast<const char*>(a.vp) + base, dma_off[j], &smem[buf][1][(first + j * RPI) * ROW]);
         }
     };
+
     int ids[GROUPS], ids_next[GROUPS];
     pages_of(k0, ids);
     if (k0 < tile_end) request(k0, ids, 0);
     pages_of(k0 + KT, ids_next);
     int buf = 0;
     for (int kt = k0; kt < tile_end; kt += KT) {
-        __syncthreads();                                   // this tile has landed, and every wave is done with the other buffer
+        // this tile has landed, and every wave is done with the other buffer
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
         const char* ks = smem[buf][0];
         char* vs = smem[buf][1];
         uint32_t absent = 0;
@@ -736,8 +773,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
         uint32_t sees[KT / 32];
         if (active) {
             t.fresh_offsets();
+            typename Tile::kfrag_t k[KT / 32];
 #pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) s[kb] = t.scores(ks, kb);
+            for (int kb = 0; kb < KT / 32; ++kb) t.load_k(ks, kb, k[kb]);
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) s[kb] = t.scores(k[kb]);
             if (absent != 0 || kt + KT > min(wave_first, tile_end)) {
 #pragma unroll
                 for (int kb = 0; kb < KT / 32; ++kb) {
@@ -770,15 +810,26 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
 #pragma unroll
                 for (int c = 0; c < Tile::kO; ++c) o[c] *= w;
             }
-            const float ref = m == -INFINITY ? 0.f : m;
+            // exp2(c x - c m) with one operation a score; far from zero, where the rounding of c m is no small number, m is
+            // taken off first
+            float mc = m == -INFINITY ? 0.f : m * a.scale_log2;
+            if (__any(!(fabsf(mc) < 16384.f))) {
+#pragma unroll
+                for (int kb = 0; kb < KT / 32; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] -= m == -INFINITY ? 0.f : m;
+                mc = 0.f;
+            }
+            float sum[4] = {l, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[kb][r] = __builtin_amdgcn_exp2f((s[kb][r] - ref) * a.scale_log2);
-                    l += s[kb][r];
+                    s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], a.scale_log2, -mc));
+                    sum[r & 3] += s[kb][r];
                 }
             }
+            l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         if (__builtin_expect(apart, 0)) {
             if (active) {
@@ -792,8 +843,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
             __syncthreads();
         }
         if (active) {
+            typename Tile::vfrag_t v[KT / 32];
 #pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) t.weigh(vs, kb, s[kb], o);
+            for (int kb = 0; kb < KT / 32; ++kb) t.load_v(vs, kb, v[kb]);
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) t.weigh(v[kb], s[kb], o);
         }
         buf ^= 1;
     }
@@ -989,7 +1043,7 @@ static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists&
         // one group of lanes for a row while the rows alone fill the chip, else eight
         const JoinArgs j{p.own.splits + p.prefix.splits, p.prefix.splits, prefix.group_starts, prefix.n};
         const int64_t heads = (int64_t)a.rows * a.hq, per = 256 / (D / 4);
-        if (heads / per >= 1024 || j.parts <= 8)
+        if (heads / per >= 256 || j.parts <= 8)
             hipLaunchKernelGGL((k_paged_join<T, D, 1>), dim3((unsigned)((heads + per - 1) / per)), dim3(256), 0, st, a, j);
         else
             hipLaunchKernelGGL((k_paged_join<T, D, 8>), dim3((unsigned)((heads + per / 8 - 1) / (per / 8))), dim3(256), 0, st, a, j);
