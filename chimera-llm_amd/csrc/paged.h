@@ -47,11 +47,14 @@ __device__ __forceinline__ int wave_count_le(const int32_t* ends, int n, int64_t
     return c;
 }
 
+constexpr int kMaxKeys = 1 << 30;    // of one list: positions a few tiles behind the last are still int32
+
 inline int check_pages(const lcmhip_kv_pages* p) {
     LCM_REQUIRE(p && p->k && p->v, "paged cache: null pages");
     LCM_REQUIRE(p->dtype == LCMHIP_F32 || p->dtype == LCMHIP_BF16, "paged cache: unknown dtype");
     LCM_REQUIRE(p->head_dim == 64 || p->head_dim == 128, "paged cache: head_dim must be 64 or 128");
-    LCM_REQUIRE(p->page_size >= 16 && (p->page_size & (p->page_size - 1)) == 0, "paged cache: page_size must be a power of two >= 16");
+    LCM_REQUIRE(p->page_size >= 16 && p->page_size <= 65536 && (p->page_size & (p->page_size - 1)) == 0,
+                "paged cache: page_size must be a power of two in [16, 65536]");
     LCM_REQUIRE(p->n_kv_heads >= 1 && p->n_kv_heads <= 65535, "paged cache: n_kv_heads out of range");
     LCM_REQUIRE(p->n_pages >= 1 && p->n_pages <= INT32_MAX, "paged cache: n_pages out of range");
     LCM_REQUIRE(((uintptr_t)p->k | (uintptr_t)p->v) % 16 == 0, "paged cache: pages must be 16-byte aligned");
@@ -63,8 +66,8 @@ inline int check_batch(const lcmhip_kv_pages* p, const lcmhip_paged_batch* b, in
     LCM_REQUIRE(b->n_seqs >= 0 && b->n_seqs <= (1 << 24), "paged batch: n_seqs out of range");
     LCM_REQUIRE(b->max_pages >= 1, "paged batch: max_pages must be positive");
     LCM_REQUIRE(b->max_q >= 1, "paged batch: max_q must be positive");
-    LCM_REQUIRE(b->max_keys >= 1 && b->max_keys <= (int64_t)b->max_pages * p->page_size,
-                "paged batch: max_keys must be in [1, max_pages * page_size]");
+    LCM_REQUIRE(b->max_keys >= 1 && b->max_keys <= kMaxKeys && b->max_keys <= (int64_t)b->max_pages * p->page_size,
+                "paged batch: max_keys must be in [1, max_pages * page_size], at most 2^30");
     LCM_REQUIRE(rows >= 0 && rows <= (1 << 30), "paged batch: rows out of range");
     LCM_REQUIRE(b->q_starts || rows == b->n_seqs, "paged batch: without q_starts there is one row for every sequence");
     return LCMHIP_OK;

@@ -465,23 +465,15 @@ struct Tile32<bf16_t, D> {
             q[st] = __builtin_bit_cast(bf16x8_t, x);
         }
     }
-    using kfrag_t = bf16x8_t[D / 16];                      // dims 16 st + 8 hi .. of row lane % 32 of a 32-key block
-    using vfrag_t = bf16x8_t[2 * kO];                      // V^T operands of its two 16-key steps
-    __device__ __forceinline__ void load_k(const char* ks, int kb, kfrag_t& k) const {
-#pragma unroll
-        for (int st = 0; st < D / 16; ++st) k[st] = *reinterpret_cast<const bf16x8_t*>(ks + kb * 32 * kRow + (k_off ^ (st << 5)));
+    __device__ __forceinline__ bf16x8_t k_operand(const char* ks, int kb, int st) const {   // dims 16 st + 8 hi .. of row lane % 32
+        return *reinterpret_cast<const bf16x8_t*>(ks + kb * 32 * kRow + (k_off ^ (st << 5)));
     }
-    __device__ __forceinline__ f32x16_t scores(const kfrag_t& k) const {
-        f32x16_t s = {};
+    __device__ __forceinline__ void scores(const char* ks, f32x16_t (&s)[2]) const {
+        s[0] = s[1] = f32x16_t{};
 #pragma unroll
-        for (int st = 0; st < D / 16; ++st) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[st], q[st], s, 0, 0, 0);
-        return s;
-    }
-    __device__ __forceinline__ void load_v(const char* vs, int kb, vfrag_t& v) const {
+        for (int st = 0; st < D / 16; ++st)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int t = 0; t < kO; ++t) v[u * kO + t] = v_operand(vs, kb, u, t);
+            for (int kb = 0; kb < 2; ++kb) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_operand(ks, kb, st), q[st], s[kb], 0, 0, 0);
     }
     __device__ __forceinline__ bf16x8_t v_operand(const char* vs, int kb, int u, int t) const {
         const char* base = vs + (kb * 32 + u * 16) * kRow;
@@ -496,13 +488,50 @@ struct Tile32<bf16_t, D> {
         for (int e = 0; e < 8; ++e) pf[e] = (__bf16)p[8 * u + e];
         return pf;
     }
-    __device__ __forceinline__ void weigh(const vfrag_t& v, const f32x16_t& p, f32x16_t (&o)[kO]) const {
+    // One tile's weights and products, and the scores of the next: s[] holds the tile's scores and next[] takes the next one's.
+    // A matrix instruction occupies its unit for 32 cycles (16 rows of 16 lanes a cycle would be 8 vector operations, 2 of them
+    // exponentials): the exponentials of the first 32 keys stand between the products of the next scores, those of the other 32
+    // between the products of the first 32 with their values, and every operand is read one product ahead.  The order is pinned;
+    // left alone the compiler puts all products before all exponentials.
+    __device__ __forceinline__ void step(const char* ks_next, const char* vs, f32x16_t (&s)[2], f32x16_t (&next)[2], float c, float mc,
+                                         float& l, f32x16_t (&o)[kO]) const {
+        constexpr int kQ = D / 8, kV = 2 * kO;             // products of the scores; of 32 keys with their values
+        constexpr int kPer = 16 / kQ, kPerV = 16 / kV;     // exponentials for each of them
+        float sum[4] = {l, 0.f, 0.f, 0.f};
+        auto weight = [&](int kb, int r) {
+            s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -mc));
+            sum[r & 3] += s[kb][r];
+        };
+        next[0] = next[1] = f32x16_t{};
+        bf16x8_t k[2];
+        k[0] = k_operand(ks_next, 0, 0);
+        bf16x8_t v[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const bf16x8_t pf = p_operand(p, u);
+        for (int i = 0; i < kQ; ++i) {
+            if (i + 1 < kQ) k[(i + 1) & 1] = k_operand(ks_next, (i + 1) & 1, (i + 1) >> 1);
+            else v[0] = v_operand(vs, 0, 0, 0);
+            next[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i & 1], q[i >> 1], next[i & 1], 0, 0, 0);
 #pragma unroll
-            for (int t = 0; t < kO; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[u * kO + t], pf, o[t], 0, 0, 0);
+            for (int x = 0; x < kPer; ++x) weight(0, i * kPer + x);
+            __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            bf16x8_t pf;
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+                const int n = kb * kV + i + 1;             // the operand read ahead
+                if (n < 2 * kV) v[n & 1] = v_operand(vs, n / kV, n % kV / kO, n % kO);
+                if (i % kO == 0) pf = p_operand(s[kb], i / kO);
+                o[i % kO] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[(n - 1) & 1], pf, o[i % kO], 0, 0, 0);
+                if (kb == 0) {
+#pragma unroll
+                    for (int x = 0; x < kPerV; ++x) weight(1, i * kPerV + x);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
     // Infinities and NaNs of a block's values for the rows that see them (bit r of `sees`: the key of register r): counted by a
     // product of ones, in which nothing can leave its row.
@@ -577,33 +606,34 @@ struct Tile32<float, D> {
             if (live) q[i] = *reinterpret_cast<const f32x4_t*>(row + 8 * i + 4 * (lane >> 5));
         }
     }
-    using kfrag_t = f32x4_t[D / 8];
-    __device__ __forceinline__ void load_k(const char* ks, int, kfrag_t& k) const {
+    __device__ __forceinline__ void scores(const char* ks, f32x16_t (&s)[1]) const {
+        s[0] = f32x16_t{};
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) k[i] = *reinterpret_cast<const f32x4_t*>(ks + (k_off ^ (i << 5)));
-    }
-    __device__ __forceinline__ f32x16_t scores(const kfrag_t& k) const {
-        f32x16_t s = {};
+        for (int i = 0; i < D / 8; ++i) {
+            const f32x4_t k = *reinterpret_cast<const f32x4_t*>(ks + (k_off ^ (i << 5)));
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i][e], q[i][e], s, 0, 0, 0);
-        return s;
+            for (int e = 0; e < 4; ++e) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[i][e], s[0], 0, 0, 0);
+        }
     }
     using piece_t = typename std::conditional<D == 128, f32x4_t, __attribute__((ext_vector_type(2))) float>::type;
     __device__ __forceinline__ piece_t v_operand(const char* vs, int r) const {      // key 8 (r / 4) + 4 hi + r % 4
         return *reinterpret_cast<const piece_t*>(vs + (8 * (r >> 2) + (r & 3)) * kRow + (v_off ^ ((8 * (r >> 2 & 1) + (r & 3)) << 4)));
     }
-    using vfrag_t = piece_t[16];
-    __device__ __forceinline__ void load_v(const char* vs, int, vfrag_t& v) const {
+    // As in bf16; 128 products of 64 cycles leave the order of the rest to the compiler.
+    __device__ __forceinline__ void step(const char* ks_next, const char* vs, f32x16_t (&s)[1], f32x16_t (&next)[1], float c, float mc,
+                                         float& l, f32x16_t (&o)[kO]) const {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = v_operand(vs, r);
-    }
-    __device__ __forceinline__ void weigh(const vfrag_t& v, const f32x16_t& p, f32x16_t (&o)[kO]) const {
+        for (int r = 0; r < 16; ++r) {
+            s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], c, -mc));
+            l += s[0][r];
+        }
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
+        for (int r = 0; r < 16; ++r) {
+            const piece_t v = v_operand(vs, r);
 #pragma unroll
-            for (int c = 0; c < kO; ++c) o[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[r][c], p[r], o[c], 0, 0, 0);
+            for (int x = 0; x < kO; ++x) o[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[x], s[0][r], o[x], 0, 0, 0);
+        }
+        scores(ks_next, next);
     }
     __device__ __forceinline__ void add_not_finite(const char* vs, int, uint32_t sees, f32x16_t (&o)[kO]) const {
 #pragma unroll
@@ -727,27 +757,35 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
         const int r = wave * (KT / 4) + j * RPI + lane / PIECES;
         dma_off[j] = (r & 15) * ROW + (((lane % PIECES) ^ Tile::swizzle(r)) << 4);
     }
-    auto request = [&](int kt, const int (&ids)[GROUPS], int buf) {
+    auto request = [&](const void* pool, int kt, const int (&ids)[GROUPS], char* dst) {
         const int first = wave * (KT / 4), id = ids[first / 16];
         const int at_group = id < 0 ? 0 : (kt + (first & ~15)) & ((1 << ls.table.page_shift) - 1);
-        const size_t base = ((((size_t)max(id, 0) * a.hk + hk) << ls.table.page_shift) + at_group) * ROW;
+        const char* base = reinterpret_cast<const char*>(pool) + ((((size_t)max(id, 0) * a.hk + hk) << ls.table.page_shift) + at_group) * ROW;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            lds_dma16(reinterpret_cast<const char*>(a.kp) + base, dma_off[j], &smem[buf][0][(first + j * RPI) * ROW]);
-            lds_dma16(reinterpret_cast<const char*>(a.vp) + base, dma_off[j], &smem[buf][1][(first + j * RPI) * ROW]);
-        }
+        for (int j = 0; j < NI; ++j) lds_dma16(base, dma_off[j], dst + (first + j * RPI) * ROW);
     };
 
-    int ids[GROUPS], ids_next[GROUPS];
-    pages_of(k0, ids);
-    if (k0 < tile_end) request(k0, ids, 0);
-    pages_of(k0 + KT, ids_next);
-    int buf = 0;
-    for (int kt = k0; kt < tile_end; kt += KT) {
-        // this tile has landed, and every wave is done with the other buffer
+    // Step i works on the scores of tile i, which step i - 1 left in registers, the values of tile i and the keys of tile i + 1;
+    // meanwhile the values of tile i + 1 and the keys of tile i + 2 arrive.  Two buffers each, one barrier a step.
+    int ids[GROUPS], ids1[GROUPS], ids2[GROUPS];           // pages of tiles i, i + 1, i + 2
+    f32x16_t s[KT / 32];
+    const float grown = 8.f / a.scale_log2;                // weights may reach 2^8 before the running maximum is moved
+    if (k0 < tile_end) {
+        pages_of(k0, ids);
+        request(a.kp, k0, ids, smem[0][0]);
+        request(a.vp, k0, ids, smem[0][1]);
+        pages_of(k0 + KT, ids1);
+        if (k0 + KT < tile_end) request(a.kp, k0 + KT, ids1, smem[1][0]);
+        pages_of(k0 + 2 * KT, ids2);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        const char* ks = smem[buf][0];
+        t.scores(smem[0][0], s);
+    }
+    int buf = 0;
+    for (int kt = k0; kt < tile_end; kt += KT) {
+        // keys i + 1 and values i have landed, and every wave is done with the buffers of keys i and values i - 1
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
         char* vs = smem[buf][1];
         uint32_t absent = 0;
 #pragma unroll
@@ -763,46 +801,44 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
             }
             apart = __syncthreads_or(apart);
         }
-        if (kt + KT < tile_end) request(kt + KT, ids_next, buf ^ 1);
+        if (kt + KT < tile_end) request(a.vp, kt + KT, ids1, smem[buf ^ 1][1]);
+        if (kt + 2 * KT < tile_end) request(a.kp, kt + 2 * KT, ids2, smem[buf][0]);
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) ids[g] = ids_next[g];
-        pages_of(kt + 2 * KT, ids_next);
+        for (int g = 0; g < GROUPS; ++g) {
+            ids[g] = ids1[g];
+            ids1[g] = ids2[g];
+        }
+        pages_of(kt + 3 * KT, ids2);
 
         const bool active = kt < wave_end;
-        f32x16_t s[KT / 32];
         uint32_t sees[KT / 32];
-        if (active) {
-            t.fresh_offsets();
-            typename Tile::kfrag_t k[KT / 32];
+        if (absent != 0 || kt + KT > min(wave_first, tile_end)) {
 #pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) t.load_k(ks, kb, k[kb]);
+            for (int kb = 0; kb < KT / 32; ++kb) {
+                sees[kb] = 0;
 #pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) s[kb] = t.scores(k[kb]);
-            if (absent != 0 || kt + KT > min(wave_first, tile_end)) {
-#pragma unroll
-                for (int kb = 0; kb < KT / 32; ++kb) {
-                    sees[kb] = 0;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = 32 * kb + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                        const bool vis = kt + i < limit && kt + i < tile_end && !(absent >> (i >> 4) & 1);
-                        if (!vis) s[kb][r] = -INFINITY;
-                        sees[kb] |= vis ? 1u << r : 0u;
-                    }
-                    seen |= sees[kb] != 0;
+                for (int r = 0; r < 16; ++r) {
+                    const int i = 32 * kb + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                    const bool vis = kt + i < limit && kt + i < tile_end && !(absent >> (i >> 4) & 1);
+                    if (!vis) s[kb][r] = -INFINITY;
+                    sees[kb] |= vis ? 1u << r : 0u;
                 }
-            } else {
-                seen = true;
-#pragma unroll
-                for (int kb = 0; kb < KT / 32; ++kb) sees[kb] = 0xffffu;
+                seen |= sees[kb] != 0;
             }
-            float top = -INFINITY;
+        } else {
+            seen |= active;
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) sees[kb] = 0xffffu;
+        }
+        if (active) {
+            float top = s[0][0];
 #pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__any(top > m)) {                          // else the running maxima stand and nothing is scaled
+            const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+            if (__any(top > m + grown)) {                  // else no weight leaves [0, 2^8] and nothing is scaled
                 const float mn = fmaxf(m, top);
                 const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
                 m = mn;
@@ -810,26 +846,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
 #pragma unroll
                 for (int c = 0; c < Tile::kO; ++c) o[c] *= w;
             }
-            // exp2(c x - c m) with one operation a score; far from zero, where the rounding of c m is no small number, m is
-            // taken off first
-            float mc = m == -INFINITY ? 0.f : m * a.scale_log2;
-            if (__any(!(fabsf(mc) < 16384.f))) {
-#pragma unroll
-                for (int kb = 0; kb < KT / 32; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] -= m == -INFINITY ? 0.f : m;
-                mc = 0.f;
-            }
-            float sum[4] = {l, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], a.scale_log2, -mc));
-                    sum[r & 3] += s[kb][r];
-                }
-            }
-            l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         if (__builtin_expect(apart, 0)) {
             if (active) {
@@ -843,11 +859,21 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
             __syncthreads();
         }
         if (active) {
-            typename Tile::vfrag_t v[KT / 32];
+            // exp2(c x - c m) with one operation a score; far from zero, where the rounding of c m is no small number, m is
+            // taken off first
+            float mc = m == -INFINITY ? 0.f : m * a.scale_log2;
+            if (__any(!(fabsf(mc) < 16384.f))) {
 #pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) t.load_v(vs, kb, v[kb]);
+                for (int kb = 0; kb < KT / 32; ++kb)
 #pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) t.weigh(v[kb], s[kb], o);
+                    for (int r = 0; r < 16; ++r) s[kb][r] -= m == -INFINITY ? 0.f : m;
+                mc = 0.f;
+            }
+            t.fresh_offsets();
+            f32x16_t next[KT / 32];
+            t.step(smem[buf ^ 1][0], vs, s, next, a.scale_log2, mc, l, o);   // behind the last tile: scores that nobody reads
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) s[kb] = next[kb];
         }
         buf ^= 1;
     }
@@ -952,8 +978,8 @@ static int check_prefix(const lcmhip_kv_pages* pages, const lcmhip_shared_prefix
     LCM_REQUIRE(prefix && prefix->page_table && prefix->lens && prefix->group_starts, "shared prefix: null argument");
     LCM_REQUIRE(prefix->n_groups >= 1 && prefix->n_groups <= (1 << 24), "shared prefix: n_groups out of range");
     LCM_REQUIRE(prefix->max_pages >= 1, "shared prefix: max_pages must be positive");
-    LCM_REQUIRE(prefix->max_keys >= 1 && prefix->max_keys <= (int64_t)prefix->max_pages * pages->page_size,
-                "shared prefix: max_keys must be in [1, max_pages * page_size]");
+    LCM_REQUIRE(prefix->max_keys >= 1 && prefix->max_keys <= kMaxKeys && prefix->max_keys <= (int64_t)prefix->max_pages * pages->page_size,
+                "shared prefix: max_keys must be in [1, max_pages * page_size], at most 2^30");
     return LCMHIP_OK;
 }
 

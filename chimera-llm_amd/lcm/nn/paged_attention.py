@@ -92,7 +92,7 @@ class HeadNorm:
 
 
 class KVPages:
-    """The page pool of one layer: k, v (pages, key heads, page_size, head_dim), contiguous; page_size a power of two >= 16."""
+    """The page pool of one layer: k, v (pages, key heads, page_size, head_dim), contiguous; page_size a power of two from 16 to 65536."""
 
     def __init__(self, k: Tensor, v: Tensor) -> None:
         _hip.require_gpu(k, "key pages")
@@ -177,7 +177,7 @@ class SharedPrefix:
 def _reach(max_keys: Optional[int], max_pages: int, pages: KVPages) -> int:
     reach = max_pages * pages.page_size
     if max_keys is None:
-        return min(reach, 2**31 - 1)
+        return min(reach, 2**30)
     if not 1 <= max_keys <= reach:
         raise ValueError(f"max_keys {max_keys} is not in [1, {reach}], what the page table holds")
     return max_keys

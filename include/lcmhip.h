@@ -415,7 +415,7 @@ int lcmhip_attention(const void* q, const void* k_cache, const void* v_cache, co
  *  - sequence lengths are cut to [0, min(max_keys, max_pages * page_size)], row ranges to [0, rows];
  *  - rows that belong to no sequence (before q_starts[0], from q_starts[n_seqs] on) are neither read nor written.
  * Row pointers are 16-byte aligned and their strides (in elements) a multiple of 16 bytes; the last dimension is dense.
- * head_dim is 64 or 128, page_size a power of two >= 16, n_heads a multiple of n_kv_heads (query head h reads key head
+ * head_dim is 64 or 128, page_size a power of two from 16 to 65536, n_heads a multiple of n_kv_heads (query head h reads key head
  * h / (n_heads / n_kv_heads)).  Outputs must not overlap inputs unless a comment says so. */
 enum { LCMHIP_NORM_NONE = -1 };                              /* lcmhip_head_norm only */
 enum { LCMHIP_ROTARY_PAIRS = 0, LCMHIP_ROTARY_HALVES = 1 };  /* pairs (2i, 2i + 1), or (i, i + rotary_dim / 2) */
@@ -436,7 +436,7 @@ typedef struct {
     const int32_t* q_starts;   /* (n_seqs + 1) or NULL: one row for every sequence */
     int32_t n_seqs, max_pages;
     int32_t max_q;             /* the most rows of one sequence; chooses the kernel, a wrong value costs time only */
-    int32_t max_keys;          /* upper bound of seq_lens, <= max_pages * page_size */
+    int32_t max_keys;          /* upper bound of seq_lens, <= max_pages * page_size and <= 2^30 */
 } lcmhip_paged_batch;
 
 /* Common beginnings: the sequences [group_starts[g], group_starts[g + 1]) continue the lens[g] positions of the pages
@@ -446,7 +446,7 @@ typedef struct {
     const int32_t* lens;         /* (n_groups) */
     const int32_t* group_starts; /* (n_groups + 1) sequence indices, not falling */
     int32_t n_groups, max_pages;
-    int32_t max_keys;            /* upper bound of lens, <= max_pages * page_size */
+    int32_t max_keys;            /* upper bound of lens, <= max_pages * page_size and <= 2^30 */
 } lcmhip_shared_prefix;
 
 /* Norm over every head (weights and biases (head_dim,) in the operand dtype, one vector for all heads; biases for

@@ -49,7 +49,7 @@ def _attend(hip, pages=None, batch=None, q=P, q_row=1024, q_head=128, out=P, row
 @pytest.mark.parametrize("kw,text", [
     (dict(k=None), b"null pages"), (dict(v=None), b"null pages"), (dict(k=P + 8), b"16-byte"), (dict(dtype=7), b"dtype"),
     (dict(head_dim=96), b"head_dim"), (dict(head_dim=256), b"head_dim"), (dict(page_size=8), b"page_size"), (dict(page_size=48), b"page_size"),
-    (dict(page_size=0), b"page_size"), (dict(n_kv_heads=0), b"n_kv_heads"), (dict(n_kv_heads=3), b"multiple of n_kv_heads"),
+    (dict(page_size=0), b"page_size"), (dict(page_size=1 << 17), b"page_size"), (dict(n_kv_heads=0), b"n_kv_heads"), (dict(n_kv_heads=3), b"multiple of n_kv_heads"),
     (dict(n_pages=0), b"n_pages"), (dict(n_pages=1 << 31), b"n_pages")])
 def test_refused_pages(hip, kw, text):
     _refused(hip, _attend(hip, pages=_pages(hip, **kw)), text)
@@ -60,7 +60,8 @@ def test_refused_pages(hip, kw, text):
 
 @pytest.mark.parametrize("kw,text", [
     (dict(page_table=None), b"null"), (dict(seq_lens=None), b"null"), (dict(n_seqs=-1), b"n_seqs"), (dict(max_pages=0), b"max_pages"),
-    (dict(max_q=0), b"max_q"), (dict(max_keys=0), b"max_keys"), (dict(max_keys=65), b"max_keys"), (dict(q_starts=None), b"one row for every sequence")])
+    (dict(max_q=0), b"max_q"), (dict(max_keys=0), b"max_keys"), (dict(max_keys=65), b"max_keys"),
+    (dict(max_keys=(1 << 30) + 1, max_pages=1 << 30), b"max_keys"), (dict(q_starts=None), b"one row for every sequence")])
 def test_refused_batches(hip, kw, text):
     _refused(hip, _attend(hip, batch=_batch(hip, **kw)), text)
     rc = hip.lib.lcmhip_paged_append(_pages(hip), _batch(hip, **kw), P, 512, 128, P, 512, 128, None, 0, 0, None, 6, 0, None, None, None, None)
