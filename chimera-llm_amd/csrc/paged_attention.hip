@@ -491,45 +491,44 @@ struct Tile32<bf16_t, D> {
     // One tile's weights and products, and the scores of the next: s[] holds the tile's scores and next[] takes the next one's.
     // A matrix instruction occupies its unit for 32 cycles (16 rows of 16 lanes a cycle would be 8 vector operations, 2 of them
     // exponentials): the exponentials of the first 32 keys stand between the products of the next scores, those of the other 32
-    // between the products of the first 32 with their values, and every operand is read one product ahead.  The order is pinned;
+    // between the products of the first 32 with their values, and every operand is read kAhead products ahead.  The order is pinned;
     // left alone the compiler puts all products before all exponentials.
     __device__ __forceinline__ void step(const char* ks_next, const char* vs, f32x16_t (&s)[2], f32x16_t (&next)[2], float c, float mc,
                                          float& l, f32x16_t (&o)[kO]) const {
         constexpr int kQ = D / 8, kV = 2 * kO;             // products of the scores; of 32 keys with their values
         constexpr int kPer = 16 / kQ, kPerV = 16 / kV;     // exponentials for each of them
+        constexpr int kAhead = 4;                          // products whose operands are read ahead: an LDS read takes longer than three
         float sum[4] = {l, 0.f, 0.f, 0.f};
         auto weight = [&](int kb, int r) {
             s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -mc));
             sum[r & 3] += s[kb][r];
         };
         next[0] = next[1] = f32x16_t{};
-        bf16x8_t k[2];
-        k[0] = k_operand(ks_next, 0, 0);
-        bf16x8_t v[2];
+        bf16x8_t ring[kAhead];
+        auto operand = [&](int n) {                        // of product n: kQ for the scores, then kV for each half of the values
+            if (n < kQ) return k_operand(ks_next, n & 1, n >> 1);
+            return v_operand(vs, (n - kQ) / kV, (n - kQ) % kV / kO, (n - kQ) % kO);
+        };
 #pragma unroll
-        for (int i = 0; i < kQ; ++i) {
-            if (i + 1 < kQ) k[(i + 1) & 1] = k_operand(ks_next, (i + 1) & 1, (i + 1) >> 1);
-            else v[0] = v_operand(vs, 0, 0, 0);
-            next[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i & 1], q[i >> 1], next[i & 1], 0, 0, 0);
+        for (int n = 0; n < kAhead; ++n) ring[n] = operand(n);
+        bf16x8_t pf;
 #pragma unroll
-            for (int x = 0; x < kPer; ++x) weight(0, i * kPer + x);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int n = 0; n < kQ + 2 * kV; ++n) {
+            if (n < kQ) {
+                next[n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[n % kAhead], q[n >> 1], next[n & 1], 0, 0, 0);
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            bf16x8_t pf;
-#pragma unroll
-            for (int i = 0; i < kV; ++i) {
-                const int n = kb * kV + i + 1;             // the operand read ahead
-                if (n < 2 * kV) v[n & 1] = v_operand(vs, n / kV, n % kV / kO, n % kO);
+                for (int x = 0; x < kPer; ++x) weight(0, n * kPer + x);
+            } else {
+                const int kb = (n - kQ) / kV, i = (n - kQ) % kV;
                 if (i % kO == 0) pf = p_operand(s[kb], i / kO);
-                o[i % kO] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[(n - 1) & 1], pf, o[i % kO], 0, 0, 0);
+                o[i % kO] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[n % kAhead], pf, o[i % kO], 0, 0, 0);
                 if (kb == 0) {
 #pragma unroll
                     for (int x = 0; x < kPerV; ++x) weight(1, i * kPerV + x);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
+            if (n + kAhead < kQ + 2 * kV) ring[n % kAhead] = operand(n + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
         }
         l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
