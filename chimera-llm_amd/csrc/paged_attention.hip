@@ -665,13 +665,17 @@ struct Tile32<float, D> {
     }
 };
 
-// 64 lanes bring 16 bytes each, from base + off (base and dst the same for the wave), to dst + 16 lane in LDS.  Written in assembly
-// because the compiler waits for every outstanding LDS-DMA before any LDS read, whatever it reads; nothing is returned in
-// registers, and the waits for the data are the loop's own (s_waitcnt vmcnt before the barrier).  M0 holds nothing across
-// instructions of the compiler.
-__device__ __forceinline__ void lds_dma16(const char* base, uint32_t off, char* dst) {
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)dst);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(off), "s"(base) : "memory");
+// 64 lanes bring 16 bytes each, from base + off[j] + 1024 j (base the same for the wave) to the 1024 bytes at LDS offset dst +
+// 1024 j, for j < N.  Written in assembly because the compiler waits for every outstanding LDS-DMA before any LDS read, whatever
+// it reads; nothing is returned in registers, and the waits for the data are the loop's own (s_waitcnt vmcnt before the
+// barrier).  M0 holds nothing across instructions of the compiler.
+template <int N>
+__device__ __forceinline__ void lds_dma(const char* base, const uint32_t (&off)[N], uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off[0]), "s"(base) : "memory");
+    if constexpr (N > 1) asm volatile("global_load_lds_dwordx4 %0, %1 offset:1024" ::"v"(off[1]), "s"(base) : "memory");
+    if constexpr (N > 2) asm volatile("global_load_lds_dwordx4 %0, %1 offset:2048" ::"v"(off[2]), "s"(base) : "memory");
+    if constexpr (N > 3) asm volatile("global_load_lds_dwordx4 %0, %1 offset:3072" ::"v"(off[3]), "s"(base) : "memory");
+    static_assert(N <= 4, "offsets are 12 bits");
 }
 
 // Many rows for each list of keys (prompts; all rows of a group against its prefix): a tile of 128 (row, head of the group)
@@ -737,45 +741,63 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
     bool seen = false;
 
     // Lane i holds the id of page page0 + i of the list: one load for 64 pages, a lane read for each use.  (Scalar loads inside
-    // the loop would make every wait for an LDS read a wait for all of them.)
-    int page0 = k0 >> ls.table.page_shift, page_ids = ls.table.page(list, (page0 + lane) << ls.table.page_shift);
-    // ids of the 16-key groups of a tile; -1 behind the last key
-    auto pages_of = [&](int kt, int (&ids)[GROUPS]) {
+    // the loop would make every wait for an LDS read a wait for all of them.)  bad: the lanes whose page is not there.
+    int page0 = k0 >> ls.table.page_shift, page_ids = 0;
+    uint64_t bad = 0;
+    auto load_ids = [&]() {
+        const int at = (page0 + lane) << ls.table.page_shift;
+        page_ids = ls.table.page(list, at);
+        bad = __ballot(page_ids < 0 && at < tile_end);
+    };
+    // Bytes from the pool's begin to the 16-key group of tile kt that holds the rows this wave brings (rows wave * KT / 4 ..); where
+    // the page is not there, to the pool's first group.
+    const int my_group = wave * (KT / 4) & ~15;
+    const uint64_t page_bytes = ((uint64_t)a.hk << ls.table.page_shift) * ROW, head_bytes = ((uint64_t)hk << ls.table.page_shift) * ROW;
+    auto source_of = [&](int kt) {
         if (((kt + KT - 1) >> ls.table.page_shift) - page0 >= 64) {
             page0 = kt >> ls.table.page_shift;
-            page_ids = ls.table.page(list, (page0 + lane) << ls.table.page_shift);
+            load_ids();
         }
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-            ids[g] = kt + 16 * g < tile_end ? __builtin_amdgcn_readlane(page_ids, ((kt + 16 * g) >> ls.table.page_shift) - page0) : -1;
+        const int key = kt + my_group, id = __builtin_amdgcn_readlane(page_ids, (key >> ls.table.page_shift) - page0);
+        const uint32_t in_page = (key & ((1 << ls.table.page_shift) - 1)) * ROW;
+        return id < 0 ? head_bytes : (uint64_t)id * page_bytes + head_bytes + in_page;
     };
-    // Wave w brings rows w KT / 4 .. of a tile, which lie in one page; the rows of a page that is not there come from page 0.
-    uint32_t dma_off[NI];
+    // the 16-key groups of tile kt whose page is not there (kt no earlier than the pages held)
+    auto absent_of = [&](int kt) {
+        uint32_t x = 0;
+        if (bad) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g)
+                x |= kt + 16 * g < tile_end && __builtin_amdgcn_readlane(page_ids, ((kt + 16 * g) >> ls.table.page_shift) - page0) < 0 ? 1u << g : 0u;
+        }
+        return x;
+    };
+    uint32_t dma_off[NI];                                  // of row j RPI + lane / PIECES behind the wave's first, less 1024 j
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
         const int r = wave * (KT / 4) + j * RPI + lane / PIECES;
-        dma_off[j] = (r & 15) * ROW + (((lane % PIECES) ^ Tile::swizzle(r)) << 4);
+        dma_off[j] = (r & 15) * ROW + (((lane % PIECES) ^ Tile::swizzle(r)) << 4) - 1024 * j;
     }
-    auto request = [&](const void* pool, int kt, const int (&ids)[GROUPS], char* dst) {
-        const int first = wave * (KT / 4), id = ids[first / 16];
-        const int at_group = id < 0 ? 0 : (kt + (first & ~15)) & ((1 << ls.table.page_shift) - 1);
-        const char* base = reinterpret_cast<const char*>(pool) + ((((size_t)max(id, 0) * a.hk + hk) << ls.table.page_shift) + at_group) * ROW;
-#pragma unroll
-        for (int j = 0; j < NI; ++j) lds_dma16(base, dma_off[j], dst + (first + j * RPI) * ROW);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)&smem[0][0][0] + wave * (KT / 4) * ROW;
+    auto request = [&](const void* pool, uint64_t source, int buf, int which) {
+        lds_dma<NI>(reinterpret_cast<const char*>(pool) + source, dma_off, lds0 + (2 * buf + which) * (KT * ROW));
     };
 
     // Step i works on the scores of tile i, which step i - 1 left in registers, the values of tile i and the keys of tile i + 1;
     // meanwhile the values of tile i + 1 and the keys of tile i + 2 arrive.  Two buffers each, one barrier a step.
-    int ids[GROUPS], ids1[GROUPS], ids2[GROUPS];           // pages of tiles i, i + 1, i + 2
     f32x16_t s[KT / 32];
     const float grown = 8.f / a.scale_log2;                // weights may reach 2^8 before the running maximum is moved
+    uint32_t absent0 = 0, absent1 = 0;                     // of tiles i and i + 1
+    uint64_t source1 = 0;                                  // of tile i + 1
     if (k0 < tile_end) {
-        pages_of(k0, ids);
-        request(a.kp, k0, ids, smem[0][0]);
-        request(a.vp, k0, ids, smem[0][1]);
-        pages_of(k0 + KT, ids1);
-        if (k0 + KT < tile_end) request(a.kp, k0 + KT, ids1, smem[1][0]);
-        pages_of(k0 + 2 * KT, ids2);
+        load_ids();
+        const uint64_t source0 = source_of(k0);
+        request(a.kp, source0, 0, 0);
+        request(a.vp, source0, 0, 1);
+        absent0 = absent_of(k0);
+        source1 = source_of(k0 + KT);
+        absent1 = absent_of(k0 + KT);
+        if (k0 + KT < tile_end) request(a.kp, source1, 1, 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         t.scores(smem[0][0], s);
@@ -786,9 +808,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         char* vs = smem[buf][1];
-        uint32_t absent = 0;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) absent |= ids[g] < 0 ? 1u << g : 0u;
+        const uint32_t absent = absent0;
         // Some keys are not there, or some rows of the workgroup do not see all of them: look for values that are not finite,
         // whose product with a weight of 0 would not be 0.
         bool apart = false;
@@ -800,14 +820,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
             }
             apart = __syncthreads_or(apart);
         }
-        if (kt + KT < tile_end) request(a.vp, kt + KT, ids1, smem[buf ^ 1][1]);
-        if (kt + 2 * KT < tile_end) request(a.kp, kt + 2 * KT, ids2, smem[buf][0]);
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            ids[g] = ids1[g];
-            ids1[g] = ids2[g];
-        }
-        pages_of(kt + 3 * KT, ids2);
+        if (kt + KT < tile_end) request(a.vp, source1, buf ^ 1, 1);
+        source1 = source_of(kt + 2 * KT);
+        absent0 = absent1;
+        absent1 = absent_of(kt + 2 * KT);
+        if (kt + 2 * KT < tile_end) request(a.kp, source1, buf, 0);
 
         const bool active = kt < wave_end;
         uint32_t sees[KT / 32];
