@@ -7,6 +7,8 @@
 //     rotation  (y_i, y_j) -> (y_i cos - y_j sin, y_i sin + y_j cos), j = i + 1 or i + rotary_dim / 2
 // in fp32, rounded once when it is stored.  The sums run over the D / 8 lanes of a head; the partner of a pair (i, i + 1) is
 // in the same lane, that of (i, i + rotary_dim / 2) rotary_dim / 16 lanes away.
+#include <algorithm>
+
 #include "paged.h"
 
 namespace lcmhip {
@@ -36,164 +38,192 @@ struct Raw8<bf16_t> { uint4 x; };
 template <>
 struct Raw8<float> { float4 x, y; };
 
-// HPT heads for each lane group; SLOTS * HPT consecutive heads (query heads, key heads, value heads of row 0, of row 1, ..)
-// for each workgroup.  All loads of a lane group's heads are in flight before the first is worked on.
-template <typename T, int D, bool APPEND, int HPT>
-__global__ __launch_bounds__(256) void k_head_rows(HeadArgs a) {
-    constexpr int LPH = D / 8, SLOTS = 256 / LPH;
-    const int nh = a.nq + a.nk + a.nv;
-    const int64_t base = (int64_t)blockIdx.x * (SLOTS * HPT);
-    const int64_t row0 = base / nh;
-    const int rem0 = (int)(base - row0 * nh);
-    const int slot = threadIdx.x / LPH, sub = threadIdx.x % LPH, i0 = sub * 8;
-    int seq0 = 0;
-    if (APPEND && a.q_starts) seq0 = wave_count_le(a.q_starts + 1, a.n_seqs, row0);
+// Value of another lane of the same 16, as an operand modifier of a vector operation (no LDS).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// Sum over the 8 or 16 lanes of a head: neighbours, pairs, mirrored halves (0xB1 / 0x4E: lane ^ 1 / ^ 2, 0x141: mirrored in 8
+// lanes, 0x140: mirrored in 16).
+template <int LPH>
+__device__ __forceinline__ float head_sum(float v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    if (LPH == 16) v += dpp<0x140>(v);
+    return v;
+}
 
-    Raw8<T> raw[HPT];
-    T* dst[HPT];
-    int kinds[HPT], poss[HPT];
-#pragma unroll
-    for (int it = 0; it < HPT; ++it) {
-        const unsigned u = (unsigned)rem0 + slot + it * SLOTS;
-        const int64_t row = row0 + u / (unsigned)nh;
-        int h = (int)(u % (unsigned)nh);
-        bool live = row < a.rows;
-        const int kind = h < a.nq ? 0 : (h < a.nq + a.nk ? 1 : 2);
-        if (kind >= 1) h -= a.nq;
-        if (kind == 2) h -= a.nk;
-        const T* src = kind == 0 ? reinterpret_cast<const T*>(a.q) + row * a.q_row + h * a.q_head
-                                 : (kind == 1 ? reinterpret_cast<const T*>(a.k) + row * a.k_row + h * a.k_head
-                                              : reinterpret_cast<const T*>(a.v) + row * a.v_row + h * a.v_head);
-        raw[it] = Raw8<T>{};
-        if (live) raw[it] = *reinterpret_cast<const Raw8<T>*>(src + i0);
-        int pos = 0;
-        T* to = nullptr;
-        if (APPEND) {
-            int c = -1, seq = seq0;
-            if (live) {
-                if (a.q_starts) {
-                    while (seq < a.n_seqs && a.q_starts[seq + 1] <= row) ++seq;   // a few rows past row0: almost never a step
-                } else {
-                    seq = (int)row;
-                }
-                if (seq < a.n_seqs) {
-                    int64_t r0, r1;
-                    seq_rows(a.q_starts, seq, a.rows, r0, r1);
-                    const int len = max(0, min(a.seq_lens[seq], a.max_keys));
-                    if (row >= r0) c = (int)max((int64_t)-1, len - (r1 - row));
-                }
-            }
-            pos = a.positions && live ? a.positions[row] : c;
-            live = c >= 0 && pos >= 0;
-            if (live && kind >= 1) {
-                const int page = a.table.page(seq, c);
-                if (page >= 0) {
-                    const int off = c & ((1 << a.table.page_shift) - 1);
-                    T* pool = reinterpret_cast<T*>(kind == 1 ? a.k_pages : a.v_pages);
-                    to = pool + ((((size_t)page * a.nk + h) << a.table.page_shift) + off) * D + i0;
-                }
-            } else if (live) {
-                to = reinterpret_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head + i0;
-            }
-        } else if (live) {
-            pos = a.positions ? a.positions[row] : 0;
-            if (pos >= 0)
-                to = kind == 0 ? reinterpret_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head + i0
-                               : reinterpret_cast<T*>(a.k_out) + row * a.ko_row + h * a.ko_head + i0;
+// A lane group keeps one row -- its place in the cache and its angles are looked up once -- and takes every (1 << head_shift)-th
+// head of the workgroup's share of heads, CHUNK of them with their loads in flight together.
+template <typename T, int D, bool APPEND, int CHUNK>
+__global__ __launch_bounds__(256) void k_head_rows(HeadArgs a, int head_shift, int heads_per_block) {
+    constexpr int LPH = D / 8, SLOTS = 256 / LPH;
+    const int slot = threadIdx.x / LPH, i0 = (threadIdx.x % LPH) * 8;
+    const int hs = 1 << head_shift, nh = a.nq + a.nk + a.nv;
+    const int64_t block_row = (int64_t)blockIdx.x * (SLOTS >> head_shift);
+    const int64_t r = block_row + (slot >> head_shift);
+    bool live = r < a.rows;
+    const int row = live ? (int)r : 0;
+    int h = blockIdx.y * heads_per_block + (slot & (hs - 1));
+    const int h1 = min(nh, (int)(blockIdx.y + 1) * heads_per_block);
+
+    int pos = 0, page = -1;
+    size_t in_pool = 0;                                    // of key head 0 at this row's place
+    if (APPEND) {
+        int seq = row;
+        if (a.q_starts) {
+            seq = wave_count_le(a.q_starts + 1, a.n_seqs, block_row);
+            while (seq < a.n_seqs && a.q_starts[seq + 1] <= row) ++seq;   // a few rows behind block_row: rarely a step
         }
-        dst[it] = to;
-        kinds[it] = kind;
-        poss[it] = pos;
+        const bool owned = live && seq < a.n_seqs;
+        const int b = owned ? seq : 0;
+        int64_t r0, r1;
+        seq_rows(a.q_starts, b, a.rows, r0, r1);
+        const int len = max(0, min(a.seq_lens[b], a.max_keys));
+        const int c = (int)max((int64_t)-1, len - (r1 - row));
+        pos = a.positions ? a.positions[row] : c;
+        live = owned && row >= r0 && c >= 0 && pos >= 0;
+        page = a.table.page(b, live ? c : 0);
+        in_pool = ((((size_t)max(page, 0) * a.nk) << a.table.page_shift) + (c & ((1 << a.table.page_shift) - 1))) * D + i0;
+    } else {
+        pos = a.positions ? a.positions[row] : 0;
+        live = live && pos >= 0;
     }
+
+    // angles: cos / sin of the lane's four pairs (i, i + 1), or of its eight dimensions whose partners are half a rotation away
+    const int half = a.rot.rotary_dim >> 1;
+    const bool turns = i0 < a.rot.rotary_dim, pairs = a.rot.style == LCMHIP_ROTARY_PAIRS, first = i0 < half;
+    const int lane = threadIdx.x & 63, partner = turns ? lane + (first ? half / 8 : -(half / 8)) : lane;
+    float cs[8] = {}, sn[8] = {};
+    if (turns) {
+        const size_t at = (size_t)min(max(pos, 0), a.rot.n_positions - 1) * half + (pairs ? i0 >> 1 : (first ? i0 : i0 - half));
+        if (pairs) {
+            *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(a.rot.cos + at);
+            *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(a.rot.sin + at);
+        } else {
+            load8<float>(a.rot.cos + at, cs);
+            load8<float>(a.rot.sin + at, sn);
 #pragma unroll
-    for (int it = 0; it < HPT; ++it) {
-        if (kinds[it] == 2) {                              // values go as they are
-            if (dst[it]) *reinterpret_cast<Raw8<T>*>(dst[it]) = raw[it];
-            continue;
+            for (int j = 0; j < 8; ++j) sn[j] = first ? -sn[j] : sn[j];
         }
+    }
+
+    auto transform = [&](const Raw8<T>& raw, const float (&w)[8], const void* bias, T* dst) {
         float x[8];
-        load8<T>(reinterpret_cast<const T*>(&raw[it]), x);
+        load8<T>(reinterpret_cast<const T*>(&raw), x);
         if (a.norm.kind != LCMHIP_NORM_NONE) {
             if (a.norm.kind != LCMHIP_NORM_RMS) {
                 float s = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) s += x[j];
+                s = head_sum<LPH>(s) * (1.f / D);
 #pragma unroll
-                for (int off = LPH / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] -= s * (1.f / D);
+                for (int j = 0; j < 8; ++j) x[j] -= s;
             }
             float s2 = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) s2 += x[j] * x[j];
+            const float r = __builtin_amdgcn_rsqf(head_sum<LPH>(s2) * (1.f / D) + a.norm.eps);   // off by no more than 2^-23
 #pragma unroll
-            for (int off = LPH / 2; off > 0; off >>= 1) s2 += __shfl_xor(s2, off, 64);
-            const float r = 1.f / sqrtf(s2 * (1.f / D) + a.norm.eps);
+            for (int j = 0; j < 8; ++j) x[j] = x[j] * r * w[j];
+            if (bias) {
+                float t[8];
+                load8<T>(reinterpret_cast<const T*>(bias) + i0, t);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= r;
-            const void* w = kinds[it] == 0 ? a.norm.q_weight : a.norm.k_weight;
-            const void* b = kinds[it] == 0 ? a.norm.q_bias : a.norm.k_bias;
-            if (w) {
-                float wv[8];
-                load8<T>(reinterpret_cast<const T*>(w) + i0, wv);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= wv[j];
-            }
-            if (b) {
-                float bv[8];
-                load8<T>(reinterpret_cast<const T*>(b) + i0, bv);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] += bv[j];
+                for (int j = 0; j < 8; ++j) x[j] += t[j];
             }
         }
         if (a.rot.rotary_dim > 0) {
-            const int half = a.rot.rotary_dim >> 1, pos = poss[it];
-            const bool known = pos < a.rot.n_positions;
-            const size_t trow = (size_t)(known ? max(pos, 0) : 0) * half;
-            if (a.rot.style == LCMHIP_ROTARY_PAIRS) {
-                if (i0 < a.rot.rotary_dim) {
-                    const float4 cs = *reinterpret_cast<const float4*>(a.rot.cos + trow + i0 / 2);
-                    const float4 sn = *reinterpret_cast<const float4*>(a.rot.sin + trow + i0 / 2);
-                    rope_rotate(x[0], x[1], cs.x, sn.x);
-                    rope_rotate(x[2], x[3], cs.y, sn.y);
-                    rope_rotate(x[4], x[5], cs.z, sn.z);
-                    rope_rotate(x[6], x[7], cs.w, sn.w);
+            if (pairs) {
+                if (turns) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) rope_rotate(x[2 * j], x[2 * j + 1], cs[j], sn[j]);
                 }
             } else {
-                const bool first = i0 < half;
-                const int lane = threadIdx.x & 63;
-                const int partner = i0 < a.rot.rotary_dim ? lane + (first ? half / 8 : -(half / 8)) : lane;
                 float y[8];
+                if (LPH == 16 && half == 64) {             // eight lanes away: half a turn of the 16
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = __shfl(x[j], partner, 64);
-                if (i0 < a.rot.rotary_dim) {
-                    float cs[8], sn[8];
-                    load8<float>(a.rot.cos + trow + (first ? i0 : i0 - half), cs);
-                    load8<float>(a.rot.sin + trow + (first ? i0 : i0 - half), sn);
+                    for (int j = 0; j < 8; ++j) y[j] = dpp<0x128>(x[j]);
+                } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = first ? x[j] * cs[j] - y[j] * sn[j] : x[j] * cs[j] + y[j] * sn[j];
+                    for (int j = 0; j < 8; ++j) y[j] = __shfl(x[j], partner, 64);
+                }
+                if (turns) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = x[j] * cs[j] + y[j] * sn[j];
                 }
             }
-            if (!known) {
+            if (pos >= a.rot.n_positions) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = __builtin_nanf("");
             }
         }
-        if (dst[it]) store8<T>(dst[it], x);
+        if (dst) store8<T>(dst, x);
+    };
+    // heads [h, end) of one kind: from `src` (of head 0 of the kind, which is head `base` of the row) to `dst`
+    auto heads = [&](int end, int base, const void* src, int64_t src_row, int64_t src_head, T* dst, int64_t dst_head, bool value,
+                     const void* weight, const void* bias) {
+        end = min(end, h1);
+        const T* from = reinterpret_cast<const T*>(src) + row * src_row + i0;
+        float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        if (weight) load8<T>(reinterpret_cast<const T*>(weight) + i0, w);
+        for (; h < end; h += CHUNK * hs) {
+            Raw8<T> raw[CHUNK];
+#pragma unroll
+            for (int it = 0; it < CHUNK; ++it) {
+                raw[it] = Raw8<T>{};
+                if (h + it * hs < end) raw[it] = *reinterpret_cast<const Raw8<T>*>(from + (h + it * hs - base) * src_head);
+            }
+#pragma unroll
+            for (int it = 0; it < CHUNK; ++it) {
+                if (h + it * hs >= end) {                  // the same for all lanes of a head
+                    h += it * hs;                          // the next kind begins here
+                    return;
+                }
+                T* to = dst ? dst + (h + it * hs - base) * dst_head : nullptr;
+                if (!value) transform(raw[it], w, bias, to);
+                else if (to) *reinterpret_cast<Raw8<T>*>(to) = raw[it];
+            }
+        }
+    };
+    T* k_dst;
+    int64_t k_dst_head;
+    if (APPEND) {
+        k_dst = live && page >= 0 ? reinterpret_cast<T*>(a.k_pages) + in_pool : nullptr;
+        k_dst_head = (int64_t)D << a.table.page_shift;
+    } else {
+        k_dst = live ? reinterpret_cast<T*>(a.k_out) + row * a.ko_row + i0 : nullptr;
+        k_dst_head = a.ko_head;
     }
+    heads(a.nq, 0, a.q, a.q_row, a.q_head, live ? reinterpret_cast<T*>(a.q_out) + row * a.qo_row + i0 : nullptr, a.qo_head, false,
+          a.norm.q_weight, a.norm.q_bias);
+    heads(a.nq + a.nk, a.nq, a.k, a.k_row, a.k_head, k_dst, k_dst_head, false, a.norm.k_weight, a.norm.k_bias);
+    if (APPEND)
+        heads(nh, a.nq + a.nk, a.v, a.v_row, a.v_head, live && page >= 0 ? reinterpret_cast<T*>(a.v_pages) + in_pool : nullptr, k_dst_head,
+              true, nullptr, nullptr);
 }
 
 template <typename T, int D, bool APPEND>
 static int launch_head_rows_t(const HeadArgs& a, hipStream_t st) {
-    constexpr int SLOTS = 256 / (D / 8);
-    const int64_t heads = a.rows * (a.nq + a.nk + a.nv);
-    if (heads == 0) return LCMHIP_OK;
-    // four heads a lane group once that still fills the chip's 256 CUs with eight workgroups each, else one
-    const int hpt = heads >= (int64_t)SLOTS * 4 * 2048 ? 4 : 1;
-    const int64_t blocks = (heads + SLOTS * hpt - 1) / (SLOTS * hpt);
-    LCM_REQUIRE(blocks <= INT32_MAX, "head rows: too many rows");
-    if (hpt == 4) hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    constexpr int SLOTS = 256 / (D / 8), WAVE_SLOTS = SLOTS / 4;
+    const int nh = a.nq + a.nk + a.nv;
+    if (a.rows == 0 || nh == 0) return LCMHIP_OK;
+    // neighbouring heads in a wave: as many as leave fewest lane groups without one
+    int shift = 0;
+    auto rounded = [&](int s) { return ((nh + (1 << s) - 1) >> s) << s; };
+    for (int s = 1; (1 << s) <= WAVE_SLOTS; ++s)
+        if (rounded(s) <= rounded(shift)) shift = s;
+    // a row's heads in one workgroup once the rows alone give the 256 CUs four workgroups each, else shared out over more
+    const int64_t blocks = (a.rows + (SLOTS >> shift) - 1) / (SLOTS >> shift);
+    const int turns = rounded(shift) >> shift;             // heads of a lane group, if one workgroup has them all
+    int64_t shares = std::min<int64_t>(turns, std::max<int64_t>(1, 1024 / blocks));
+    const int each = (int)((turns + shares - 1) / shares);
+    shares = (turns + each - 1) / each;
+    LCM_REQUIRE(blocks <= INT32_MAX && shares <= 65535, "head rows: too many rows or heads");
+    const dim3 grid((unsigned)blocks, (unsigned)shares);
+    if (each > 1) hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 4>), grid, dim3(256), 0, st, a, shift, each << shift);
+    else hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 1>), grid, dim3(256), 0, st, a, shift, each << shift);
     LCM_HIP_CHECK(hipGetLastError());
     return LCMHIP_OK;
 }
