@@ -27,6 +27,7 @@ struct KeyLists {
     int n, max_keys;
     int causal;                      // row r of the list sees keys [0, len - rows + r + 1)
     int splits, part0;               // parts of a list, and the number of the first
+    int many, tiles;                 // many_rows(): tiles in all; few_rows(): tiles a list
 };
 
 struct PagedArgs {
@@ -257,15 +258,17 @@ struct Tile16<float, D> {
 
 // Few rows for each list of keys: a tile of 16 (row, head of the group) pairs of one key head against one part of a list, four
 // waves that take the part's groups of keys in turn and join their results in LDS.  Bound by the bytes of the keys and values.
+template <int D>
+struct FewShared {
+    float o[4][16][D + 4];
+    float2 ml[4][16];
+};
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void k_paged_few(PagedArgs a, KeyLists ls, int row_tiles) {
+__device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls, int bid, FewShared<D>& red) {
     using Tile = Tile16<T, D>;
-    constexpr int NP = 4 * Tile::kHalves, OROW = D + 4;
-    __shared__ float red_o[4][16][OROW];
-    __shared__ float2 red_ml[4][16];
+    constexpr int NP = 4 * Tile::kHalves;
     const int lane = threadIdx.x & 63, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int bid = blockIdx.x;
     const int hk = bid % a.hk;
     bid /= a.hk;
     const int split = bid % ls.splits;
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedArgs a, KeyLists ls, 
     const T* kp = reinterpret_cast<const T*>(a.kp);
     const T* vp = reinterpret_cast<const T*>(a.vp);
 
-    for (int t0 = tile0 * 16; t0 < n_rows; t0 += row_tiles * 16) {
+    for (int t0 = tile0 * 16; t0 < n_rows; t0 += ls.tiles * 16) {
         const int mine = t0 + (lane & 15);                 // (row, head) pair of this lane
         const bool live = mine < n_rows;
         const int row = r0 + (live ? mine / G : 0);
@@ -387,23 +390,23 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedArgs a, KeyLists ls, 
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int c = 0; c < Tile::kO; ++c) red_o[wave][lane & 15][Tile::dim(c, r, lane)] = o[c][r];
-        if (quad == 0) red_ml[wave][lane & 15] = make_float2(m, l);
+            for (int c = 0; c < Tile::kO; ++c) red.o[wave][lane & 15][Tile::dim(c, r, lane)] = o[c][r];
+        if (quad == 0) red.ml[wave][lane & 15] = make_float2(m, l);
         __syncthreads();
         const int tile_rows = min(16, n_rows - t0);
         for (int i = threadIdx.x; i < tile_rows * (D / 4); i += 256) {
             const int x = i / (D / 4), d4 = i % (D / 4) * 4;
             float M = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) M = fmaxf(M, red_ml[w][x].x);
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, red.ml[w][x].x);
             float L = 0.f;
             f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float2 ml = red_ml[w][x];
+                const float2 ml = red.ml[w][x];
                 const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * a.scale_log2);
                 L += ml.y * f;
-                acc += *reinterpret_cast<const f32x4_t*>(&red_o[w][x][d4]) * f;
+                acc += *reinterpret_cast<const f32x4_t*>(&red.o[w][x][d4]) * f;
             }
             const size_t at = (size_t)(r0 + (t0 + x) / G) * a.hq + hk * G + (t0 + x) % G;
             if (a.part_o) {
@@ -682,21 +685,24 @@ __device__ __forceinline__ void lds_dma(const char* base, const uint32_t (&off)[
 // pairs of one key head against one part of a list; wave w has pairs 32 w .., and the four share the keys and values that
 // LDS-DMA brings one tile ahead.  Bound by the matrix instructions.
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls, int tiles) {
+struct ManyShared {
+    char kv[2][2][Tile32<T, D>::kKeys * Tile32<T, D>::kRow];   // [buffer][keys, values]
+};
+template <typename T, int D>
+__device__ __forceinline__ void many_rows(const PagedArgs& a, const KeyLists& ls, int bid, ManyShared<T, D>& shared) {
     using Tile = Tile32<T, D>;
     constexpr int KT = Tile::kKeys, ROW = Tile::kRow, PIECES = ROW / 16, GROUPS = KT / 16;
     constexpr int RPI = 1024 / ROW, NI = KT / 4 / RPI;     // rows of one DMA instruction, instructions of a wave for a tile
-    __shared__ __attribute__((aligned(1024))) char smem[2][2][KT * ROW];
+    auto& smem = shared.kv;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.hq / a.hk;
-    int bid = blockIdx.x;
     const int hk = bid % a.hk;                             // workgroups of one key head meet in the same L2 (8 XCDs, dealt in turn)
     bid /= a.hk;
     const int split = bid % ls.splits;
     // Tiles are numbered so that list i has those from floor(r0 G / 128) + i on, which leaves every list as many as it needs.
     // Late tiles first: under a causal mask they have the most keys.
-    const int tile = tiles - 1 - bid / ls.splits;
+    const int tile = ls.tiles - 1 - bid / ls.splits;
     int list = 0;
     {
         int c = 0;
@@ -909,6 +915,34 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls,
     }
 }
 
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void k_paged_few(PagedArgs a, KeyLists ls) {
+    __shared__ FewShared<D> shared;
+    few_rows<T, D>(a, ls, blockIdx.x, shared);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls) {
+    __shared__ __attribute__((aligned(1024))) ManyShared<T, D> shared;
+    many_rows<T, D>(a, ls, blockIdx.x, shared);
+}
+
+// Prefixes and own positions in one launch: the prefixes' work is bound by matrix instructions where groups are large, the own
+// positions' by memory, and small calls save a launch.  Eight workgroups at a time (one for each XCD) belong to one of the two,
+// spread evenly: n0 workgroups of `prefix`, n1 of `own`.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void k_paged_pair(PagedArgs a, KeyLists prefix, KeyLists own, int n0, int n1) {
+    __shared__ __attribute__((aligned(1024))) union { FewShared<D> few; ManyShared<T, D> many; } shared;
+    const int64_t u0 = (n0 + 7) >> 3, u1 = (n1 + 7) >> 3, t = blockIdx.x >> 3;
+    const int64_t before = t * u0 / (u0 + u1);             // eights of the prefix before this one
+    const bool is_prefix = (t + 1) * u0 / (u0 + u1) > before;
+    const int bid = (int)((is_prefix ? before : t - before) << 3) + (blockIdx.x & 7);
+    if (bid >= (is_prefix ? n0 : n1)) return;
+    const KeyLists& ls = is_prefix ? prefix : own;
+    if (ls.many) many_rows<T, D>(a, ls, bid, shared.many);
+    else few_rows<T, D>(a, ls, bid, shared.few);
+}
+
 struct JoinArgs {
     int parts, prefix_parts;         // the prefix's parts come first
     const int32_t* group_starts;     // null: no prefix
@@ -1071,16 +1105,20 @@ static Plan make_plan(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* ba
 
 template <typename T, int D>
 static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists& prefix, const Plan& p, hipStream_t st) {
-    auto attend = [&](const KeyLists& ls, const ListPlan& lp) {
-        const int64_t blocks = (int64_t)a.hk * ls.splits * (lp.many ? lp.tiles : (int64_t)ls.n * lp.tiles);
-        LCM_REQUIRE(blocks <= INT32_MAX, "paged attention: too many rows");
-        if (lp.many) hipLaunchKernelGGL((k_paged_many<T, D>), dim3((unsigned)blocks), dim3(256), 0, st, a, ls, lp.tiles);
-        else hipLaunchKernelGGL((k_paged_few<T, D>), dim3((unsigned)blocks), dim3(256), 0, st, a, ls, lp.tiles);
-        LCM_HIP_CHECK(hipGetLastError());
-        return LCMHIP_OK;
-    };
-    if (prefix.n > 0) LCM_TRY(attend(prefix, p.prefix));
-    LCM_TRY(attend(own, p.own));
+    auto blocks_of = [&](const KeyLists& ls) { return (int64_t)a.hk * ls.splits * (ls.many ? ls.tiles : (int64_t)ls.n * ls.tiles); };
+    const int64_t n1 = blocks_of(own);
+    LCM_REQUIRE(n1 <= INT32_MAX / 4, "paged attention: too many rows");
+    if (prefix.n > 0) {
+        const int64_t n0 = blocks_of(prefix);
+        LCM_REQUIRE(n0 <= INT32_MAX / 4, "paged attention: too many rows");
+        hipLaunchKernelGGL((k_paged_pair<T, D>), dim3((unsigned)((((n0 + 7) >> 3) + ((n1 + 7) >> 3)) << 3)), dim3(256), 0, st, a, prefix, own,
+                           (int)n0, (int)n1);
+    } else if (own.many) {
+        hipLaunchKernelGGL((k_paged_many<T, D>), dim3((unsigned)n1), dim3(256), 0, st, a, own);
+    } else {
+        hipLaunchKernelGGL((k_paged_few<T, D>), dim3((unsigned)n1), dim3(256), 0, st, a, own);
+    }
+    LCM_HIP_CHECK(hipGetLastError());
     if (p.joined) {
         // one group of lanes for a row while the rows alone fill the chip, else eight
         const JoinArgs j{p.own.splits + p.prefix.splits, p.prefix.splits, prefix.group_starts, prefix.n};
@@ -1113,11 +1151,11 @@ static int paged_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     a.rows = (int)rows; a.hq = n_heads; a.hk = pages->n_kv_heads;
     a.scale_log2 = scale * 1.4426950408889634f;
     const KeyLists own{PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), (uint32_t)pages->n_pages}, batch->seq_lens, nullptr,
-                     batch->n_seqs, batch->max_keys, causal != 0, p.own.splits, p.prefix.splits};
+                     batch->n_seqs, batch->max_keys, causal != 0, p.own.splits, p.prefix.splits, p.own.many, p.own.tiles};
     KeyLists pre{};
     if (prefix)
         pre = KeyLists{PageTable{prefix->page_table, prefix->max_pages, page_shift_of(pages), (uint32_t)pages->n_pages}, prefix->lens,
-                            prefix->group_starts, prefix->n_groups, prefix->max_keys, 0, p.prefix.splits, 0};
+                            prefix->group_starts, prefix->n_groups, prefix->max_keys, 0, p.prefix.splits, 0, p.prefix.many, p.prefix.tiles};
     if (p.joined) {
         a.part_ml = reinterpret_cast<float2*>(ws);
         a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + p.ml_bytes);

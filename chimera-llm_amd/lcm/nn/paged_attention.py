@@ -190,21 +190,22 @@ def _grad_free(*tensors: Tensor) -> None:
                 raise RuntimeError(_NO_BACKWARD)
 
 
+def _new(like: Tensor) -> Tensor:
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
+
+
 def _heads(t: Tensor, what: str, dtype: torch.dtype, device: torch.device, rows: Optional[int], heads: Optional[int],
            head_dim: int) -> Tuple[int, int, int]:
     """(pointer, row stride, head stride) of a row tensor (rows, heads, head_dim) with a dense last dimension; None: any number.
     These checks stand in front of kernels of a few microseconds: they build no message before they fail."""
-    shape = t.shape
-    if len(shape) != 3 or t.stride(2) != 1 and shape[2] != 1:
-        raise ValueError(f"{what} must be (rows, heads, head_dim) with a dense last dimension")
-    if t.device != device:
-        _hip.require_gpu(t, what)
-        raise ValueError(f"{what} lives on {t.device}, not on {device}")
-    if (t.dtype is not dtype or shape[2] != head_dim or (heads is not None and shape[1] != heads)
-            or (rows is not None and shape[0] != rows)):
-        raise ValueError(f"{what} is {tuple(shape)} {t.dtype}, expected ({'any' if rows is None else rows}, "
-                         f"{'any' if heads is None else heads}, {head_dim}) {dtype}")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    shape, stride = t.shape, t.stride()
+    if (len(shape) == 3 and stride[2] == 1 and shape[2] == head_dim and t.dtype is dtype and t.device == device
+            and (heads is None or shape[1] == heads) and (rows is None or shape[0] == rows)):
+        return t.data_ptr(), stride[0], stride[1]
+    _hip.require_gpu(t, what)
+    raise ValueError(f"{what} is {tuple(shape)} with strides {stride}, {t.dtype} on {t.device}; expected "
+                     f"({'any' if rows is None else rows}, {'any' if heads is None else heads}, {head_dim}) with a dense last "
+                     f"dimension, {dtype} on {device}")
 
 
 def _call(device: torch.device, fn, *args) -> None:
@@ -240,18 +241,21 @@ def head_norm_rope(q: Optional[Tensor], k: Optional[Tensor], *, positions: Optio
     `positions` (rows,) int32 with `rope`: a row of a negative position is skipped (padding: q_out and k_out keep what they
     hold there), one beyond the table gives NaN.  q_out / k_out default to new contiguous tensors and may be q / k themselves."""
     like = q if q is not None else k
-    _require(like is not None, "head_norm_rope needs queries or keys")
-    _hip.require_gpu(like, "heads")
-    dtype, device = like.dtype, like.device
-    _require(like.dim() == 3, "queries and keys must be (rows, heads, head_dim)")
-    rows, _, head_dim = like.shape
+    if like is None:
+        raise ValueError("head_norm_rope needs queries or keys")
+    dtype, device, shape = like.dtype, like.device, like.shape
+    if len(shape) != 3:
+        raise ValueError("queries and keys must be (rows, heads, head_dim)")
+    if not like.is_cuda:
+        _hip.require_gpu(like, "heads")
+    rows, _, head_dim = shape
     q_args = k_args = qo_args = ko_args = (None, 0, 0)
     q_heads = k_heads = 0
     if q is not None:
         _grad_free(q)
-        q_args, q_heads = _heads(q, "q", dtype, device, rows, None, head_dim), q.shape[1]
+        q_args, q_heads = _heads(q, "q", dtype, device, rows, None, head_dim), shape[1]
         if q_out is None:
-            q_out = q.new_empty(q.shape)
+            q_out = _new(q)
             qo_args = q_out.data_ptr(), q_heads * head_dim, head_dim
         else:
             qo_args = _heads(q_out, "q_out", dtype, device, rows, q_heads, head_dim)
@@ -261,13 +265,14 @@ def head_norm_rope(q: Optional[Tensor], k: Optional[Tensor], *, positions: Optio
         _grad_free(k)
         k_args, k_heads = _heads(k, "k", dtype, device, rows, None, head_dim), k.shape[1]
         if k_out is None:
-            k_out = k.new_empty(k.shape)
+            k_out = _new(k)
             ko_args = k_out.data_ptr(), k_heads * head_dim, head_dim
         else:
             ko_args = _heads(k_out, "k_out", dtype, device, rows, k_heads, head_dim)
     elif k_out is not None:
         raise ValueError("k_out without k")
-    _require(rope is None or positions is not None, "a rotation needs positions")
+    if rope is not None and positions is None:
+        raise ValueError("a rotation needs positions")
     norm_ref, rope_ref, pos = _transform(rope, norm, positions, like)
     if rows == 0:                          # an empty tensor has no address
         return q_out, k_out
@@ -296,7 +301,7 @@ def paged_append(pages: KVPages, batch: PagedBatch, k: Tensor, v: Tensor, *, q: 
         _grad_free(q)
         qp, heads = _heads(q, "q", dtype, device, rows, None, head_dim), q.shape[1]
         if q_out is None:
-            q_out = q.new_empty(q.shape)
+            q_out = _new(q)
         else:
             _heads(q_out, "q_out", dtype, device, rows, heads, head_dim)
             _require(q_out.is_contiguous(), "q_out must be contiguous")
@@ -316,7 +321,7 @@ def _attend(q: Tensor, pages: KVPages, batch: PagedBatch, prefix: Optional[Share
     qp = _heads(q, "q", pages.dtype, pages.device, None, None, pages.head_dim)
     rows, heads, head_dim = q.shape
     if out is None:
-        out = q.new_empty(q.shape)
+        out = _new(q)
     else:
         _heads(out, "out", pages.dtype, pages.device, rows, heads, head_dim)
         _require(out.is_contiguous(), "out must be contiguous")
