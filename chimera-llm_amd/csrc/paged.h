@@ -41,9 +41,7 @@ __host__ __device__ __forceinline__ void seq_rows(const int32_t* starts, int b, 
 __device__ __forceinline__ int wave_count_le(const int32_t* ends, int n, int64_t t) {
     const int lane = threadIdx.x & 63;
     int c = 0;
-    for (int i = lane; i < n; i += 64) c += ends[i] <= t ? 1 : 0;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) c += __shfl_xor(c, off, 64);
+    for (int i = 0; i < n; i += 64) c += __popcll(__ballot(i + lane < n && ends[min(i + lane, n - 1)] <= t));
     return c;
 }
 

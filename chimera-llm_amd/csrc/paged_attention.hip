@@ -36,11 +36,15 @@ struct PagedArgs {
     const void *kp, *vp;
     const int32_t* q_starts;
     int n_seqs, rows, hq, hk;
+    int G;                     // query heads of a key head
+    uint32_t g_magic, g_shift; // x / G = (umulhi(g_magic, x) + x) >> g_shift for 0 <= x < 2^31
     float scale_log2;          // scale * log2(e).  It multiplies differences of dot products only: a product that fits fp32
                                // may leave it when multiplied by log2(e), and far from zero its rounding is no small number
     float* part_o;             // [part][row][head][D], not divided by l; null: a single part, finished in place
     float2* part_ml;           // [part][row][head] (m, l)
 };
+
+__device__ __forceinline__ int div_g(const PagedArgs& a, int x) { return (int)((__umulhi(a.g_magic, (uint32_t)x) + (uint32_t)x) >> a.g_shift); }
 
 // Rows and keys of list i.
 __device__ __forceinline__ void list_extent(const PagedArgs& a, const KeyLists& ls, int i, int& r0, int& r1, int& keys) {
@@ -274,7 +278,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
     const int split = bid % ls.splits;
     bid /= ls.splits;
     const int list = bid % ls.n, tile0 = bid / ls.n;
-    const int G = a.hq / a.hk;
+    const int G = a.G;
     int r0, r1, keys, k0, k1;
     list_extent(a, ls, list, r0, r1, keys);
     part_range<32>(keys, ls.splits, kMinPartFew, split, k0, k1);
@@ -285,12 +289,12 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
     for (int t0 = tile0 * 16; t0 < n_rows; t0 += ls.tiles * 16) {
         const int mine = t0 + (lane & 15);                 // (row, head) pair of this lane
         const bool live = mine < n_rows;
-        const int row = r0 + (live ? mine / G : 0);
-        const int head = hk * G + (live ? mine % G : 0);
+        const int token = live ? div_g(a, mine) : 0, row = r0 + token;
+        const int head = hk * G + (live ? mine - token * G : 0);
         // keys that this row and the tile's first row see (later rows see no fewer)
         const int limit = ls.causal ? keys - (r1 - row) + 1 : keys;
-        const int first_limit = ls.causal ? keys - (r1 - r0 - t0 / G) + 1 : keys;
-        const int last_limit = ls.causal ? keys - (r1 - r0 - min(t0 + 15, n_rows - 1) / G) + 1 : keys;
+        const int first_limit = ls.causal ? keys - (r1 - r0 - div_g(a, t0)) + 1 : keys;
+        const int last_limit = ls.causal ? keys - (r1 - r0 - div_g(a, min(t0 + 15, n_rows - 1))) + 1 : keys;
         const int end = min(k1, last_limit);
 
         Tile t;
@@ -408,7 +412,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
                 L += ml.y * f;
                 acc += *reinterpret_cast<const f32x4_t*>(&red.o[w][x][d4]) * f;
             }
-            const size_t at = (size_t)(r0 + (t0 + x) / G) * a.hq + hk * G + (t0 + x) % G;
+            const int token = div_g(a, t0 + x);
+            const size_t at = (size_t)(r0 + token) * a.hq + hk * G + (t0 + x - token * G);
             if (a.part_o) {
                 const size_t part = (size_t)(ls.part0 + split) * ((size_t)a.rows * a.hq) + at;
                 *reinterpret_cast<f32x4_t*>(a.part_o + part * D + d4) = acc;
@@ -696,30 +701,29 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const KeyLists& ls
     auto& smem = shared.kv;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int G = a.hq / a.hk;
+    const int G = a.G;
     const int hk = bid % a.hk;                             // workgroups of one key head meet in the same L2 (8 XCDs, dealt in turn)
     bid /= a.hk;
     const int split = bid % ls.splits;
     // Tiles are numbered so that list i has those from floor(r0 G / 128) + i on, which leaves every list as many as it needs.
     // Late tiles first: under a causal mask they have the most keys.
     const int tile = ls.tiles - 1 - bid / ls.splits;
-    int list = 0;
-    {
-        int c = 0;
-        for (int i = lane; i < ls.n; i += 64) {
-            int s1 = i + 1;
-            if (ls.group_starts) s1 = min(max(ls.group_starts[i + 1], 0), a.n_seqs);
-            int r1 = a.q_starts ? a.q_starts[s1] : s1;
-            r1 = min(max(r1, 0), a.rows);
-            c += (int)((int64_t)r1 * G >> 7) + i + 1 <= tile ? 1 : 0;
+    // 64 lists at a time, a lane each; the first whose tiles do not end before this one
+    int list = -1, r0 = 0, r1 = 0, keys = 0, k0, k1;
+    for (int first = 0; first < ls.n; first += 64) {
+        int x0 = 0, x1 = 0, xk = 0;
+        const bool is_list = first + lane < ls.n;
+        if (is_list) list_extent(a, ls, first + lane, x0, x1, xk);
+        const int c = __popcll(__ballot(is_list && (int)((int64_t)x1 * G >> 7) + first + lane + 1 <= tile));
+        if (c < min(64, ls.n - first)) {
+            list = first + c;
+            r0 = __builtin_amdgcn_readlane(x0, c);
+            r1 = __builtin_amdgcn_readlane(x1, c);
+            keys = __builtin_amdgcn_readlane(xk, c);
+            break;
         }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) c += __shfl_xor(c, off, 64);
-        list = __builtin_amdgcn_readfirstlane(c);
     }
-    if (list >= ls.n) return;
-    int r0, r1, keys, k0, k1;
-    list_extent(a, ls, list, r0, r1, keys);
+    if (list < 0) return;
     part_range<KT>(keys, ls.splits, 2 * KT, split, k0, k1);
     const int n_rows = (r1 - r0) * G;
     const int t0 = (tile - (int)((int64_t)r0 * G >> 7) - list) * 128;
@@ -727,15 +731,15 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const KeyLists& ls
 
     const int mine = t0 + 32 * wave + (lane & 31);
     const bool live = mine < n_rows;
-    const int row = r0 + (live ? mine / G : 0);
-    const int head = hk * G + (live ? mine % G : 0);
+    const int token = live ? div_g(a, mine) : 0, row = r0 + token;
+    const int head = hk * G + (live ? mine - token * G : 0);
     const int at_end = keys - (r1 - r0) + 1;               // keys that the list's first row sees
     const int limit = ls.causal ? keys - (r1 - row) + 1 : keys;
-    const int tile_end = min(k1, ls.causal ? at_end + min(t0 + 127, n_rows - 1) / G : keys);
-    const int tile_first = ls.causal ? at_end + t0 / G : keys;
+    const int tile_end = min(k1, ls.causal ? at_end + div_g(a, min(t0 + 127, n_rows - 1)) : keys);
+    const int tile_first = ls.causal ? at_end + div_g(a, t0) : keys;
     const bool wave_live = t0 + 32 * wave < n_rows;
-    const int wave_first = ls.causal ? at_end + (t0 + 32 * wave) / G : keys;
-    const int wave_end = !wave_live ? 0 : min(k1, ls.causal ? at_end + min(t0 + 32 * wave + 31, n_rows - 1) / G : keys);
+    const int wave_first = ls.causal ? at_end + div_g(a, t0 + 32 * wave) : keys;
+    const int wave_end = !wave_live ? 0 : min(k1, ls.causal ? at_end + div_g(a, min(t0 + 32 * wave + 31, n_rows - 1)) : keys);
 
     Tile t;
     t.init(lane);
@@ -1148,7 +1152,9 @@ static int paged_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     PagedArgs a{};
     a.q = q; a.q_row = q_row; a.q_head = q_head; a.out = out; a.kp = pages->k; a.vp = pages->v;
     a.q_starts = batch->q_starts; a.n_seqs = batch->n_seqs;
-    a.rows = (int)rows; a.hq = n_heads; a.hk = pages->n_kv_heads;
+    a.rows = (int)rows; a.hq = n_heads; a.hk = pages->n_kv_heads; a.G = n_heads / pages->n_kv_heads;
+    while ((1 << a.g_shift) < a.G) ++a.g_shift;
+    a.g_magic = (uint32_t)((((uint64_t)1 << 32) * ((1u << a.g_shift) - a.G)) / a.G + 1);
     a.scale_log2 = scale * 1.4426950408889634f;
     const KeyLists own{PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), (uint32_t)pages->n_pages}, batch->seq_lens, nullptr,
                      batch->n_seqs, batch->max_keys, causal != 0, p.own.splits, p.prefix.splits, p.own.many, p.own.tiles};
