@@ -28,6 +28,7 @@ struct KeyLists {
     int causal;                      // row r of the list sees keys [0, len - rows + r + 1)
     int splits, part0;               // parts of a list, and the number of the first
     int many, tiles;                 // many_rows(): tiles in all; few_rows(): tiles a list
+    int alone;                       // few_rows(): every wave has a part of its own (short parts), or four waves share one
 };
 
 struct PagedArgs {
@@ -78,6 +79,12 @@ __device__ __forceinline__ void part_range(int keys, int splits, int least, int 
 // The order of the inner index is free as long as both operands agree: key slots are numbered so that the operand P^T is
 // what the lane holds, and dim rows so that the operand V^T is what 16-byte loads of value rows bring (below).
 // No operand passes through LDS, and consecutive lanes read consecutive bytes.
+__device__ __forceinline__ void store4(float* p, f32x4_t x) { *reinterpret_cast<f32x4_t*>(p) = x; }
+__device__ __forceinline__ void store4(bf16_t* p, f32x4_t x) {
+    *reinterpret_cast<u32x2_t*>(p) = u32x2_t{(uint32_t)f32_to_bf16(x[0]) | ((uint32_t)f32_to_bf16(x[1]) << 16),
+                                             (uint32_t)f32_to_bf16(x[2]) | ((uint32_t)f32_to_bf16(x[3]) << 16)};
+}
+
 // Mask of the bf16 halves of a word that are NaN or infinite.
 __device__ __forceinline__ uint32_t not_finite(uint32_t x) {
     return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
@@ -273,6 +280,11 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
     constexpr int NP = 4 * Tile::kHalves;
     const int lane = threadIdx.x & 63, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int stride = ls.alone ? Tile::kKeys : 4 * Tile::kKeys;   // from one group of keys of this wave to the next
+    if (ls.alone) {
+        bid = 4 * bid + wave;
+        if (bid >= a.hk * ls.splits * ls.n * ls.tiles) return;     // no barrier below
+    }
     const int hk = bid % a.hk;
     bid /= a.hk;
     const int split = bid % ls.splits;
@@ -313,17 +325,17 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
         };
         size_t off[2], off_next[2];
         int there[2], there_next[2];
-        int key = k0 + wave * Tile::kKeys;
+        int key = k0 + (ls.alone ? 0 : wave * Tile::kKeys);
 #pragma unroll
         for (int h = 0; h < Tile::kHalves; ++h) {
             place(key + 16 * h, off[h], there[h]);
             if (key < end) t.load_k(h, kp + off[h], lane);
         }
-        for (; key < end; key += 4 * Tile::kKeys) {
+        for (; key < end; key += stride) {
             // the values of this group and the keys of the next are in flight while the scores are worked out
 #pragma unroll
             for (int h = 0; h < Tile::kHalves; ++h) t.load_v(h, vp + off[h], lane);
-            const int next = key + 4 * Tile::kKeys;
+            const int next = key + stride;
 #pragma unroll
             for (int h = 0; h < Tile::kHalves; ++h) place(next + 16 * h, off_next[h], there_next[h]);
             float s[NP];
@@ -396,17 +408,17 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
 #pragma unroll
             for (int c = 0; c < Tile::kO; ++c) red.o[wave][lane & 15][Tile::dim(c, r, lane)] = o[c][r];
         if (quad == 0) red.ml[wave][lane & 15] = make_float2(m, l);
-        __syncthreads();
-        const int tile_rows = min(16, n_rows - t0);
-        for (int i = threadIdx.x; i < tile_rows * (D / 4); i += 256) {
+        // the waves' results of a row together, or this wave's alone (LDS operations of one wave keep their order)
+        if (ls.alone) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        else __syncthreads();
+        const int tile_rows = min(16, n_rows - t0), w0 = ls.alone ? wave : 0, w1 = ls.alone ? wave + 1 : 4;
+        for (int i = ls.alone ? lane : threadIdx.x; i < tile_rows * (D / 4); i += ls.alone ? 64 : 256) {
             const int x = i / (D / 4), d4 = i % (D / 4) * 4;
             float M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) M = fmaxf(M, red.ml[w][x].x);
+            for (int w = w0; w < w1; ++w) M = fmaxf(M, red.ml[w][x].x);
             float L = 0.f;
             f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = w0; w < w1; ++w) {
                 const float2 ml = red.ml[w][x];
                 const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * a.scale_log2);
                 L += ml.y * f;
@@ -419,12 +431,11 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
                 *reinterpret_cast<f32x4_t*>(a.part_o + part * D + d4) = acc;
                 if (d4 == 0) a.part_ml[part] = make_float2(M, L);
             } else {
-                T* dst = reinterpret_cast<T*>(a.out) + at * D + d4;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) Elem<T>::store(dst + e, M == -INFINITY ? 0.f : acc[e] / L);
+                store4(reinterpret_cast<T*>(a.out) + at * D + d4, M == -INFINITY ? f32x4_t{0.f, 0.f, 0.f, 0.f} : acc / L);
             }
         }
-        __syncthreads();
+        if (ls.alone) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        else __syncthreads();
     }
 }
 
@@ -931,16 +942,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PagedArgs a, KeyLists ls)
     many_rows<T, D>(a, ls, blockIdx.x, shared);
 }
 
-// Prefixes and own positions in one launch: the prefixes' work is bound by matrix instructions where groups are large, the own
-// positions' by memory, and small calls save a launch.  Eight workgroups at a time (one for each XCD) belong to one of the two,
-// spread evenly: n0 workgroups of `prefix`, n1 of `own`.
+// Prefixes and own positions in one launch: small calls save one, and in large ones the prefixes, bound by matrix instructions, share
+// the chip with own positions, bound by memory, as they run out.  n0 workgroups of `prefix`, then (from a multiple of 8 on: the
+// XCDs are dealt in turn) n1 of `own`.  Spreading the two evenly instead took 225 us against 207 (192 continuations of four
+// prefixes of 20k-32k positions).
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void k_paged_pair(PagedArgs a, KeyLists prefix, KeyLists own, int n0, int n1) {
     __shared__ __attribute__((aligned(1024))) union { FewShared<D> few; ManyShared<T, D> many; } shared;
-    const int64_t u0 = (n0 + 7) >> 3, u1 = (n1 + 7) >> 3, t = blockIdx.x >> 3;
-    const int64_t before = t * u0 / (u0 + u1);             // eights of the prefix before this one
-    const bool is_prefix = (t + 1) * u0 / (u0 + u1) > before;
-    const int bid = (int)((is_prefix ? before : t - before) << 3) + (blockIdx.x & 7);
+    const int first_own = (n0 + 7) & ~7;
+    const bool is_prefix = (int)blockIdx.x < first_own;
+    const int bid = is_prefix ? blockIdx.x : blockIdx.x - first_own;
     if (bid >= (is_prefix ? n0 : n1)) return;
     const KeyLists& ls = is_prefix ? prefix : own;
     if (ls.many) many_rows<T, D>(a, ls, bid, shared.many);
@@ -1022,9 +1033,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, JoinArgs j) {
         m = M;
     }
     if (live) {
-        T* dst = reinterpret_cast<T*>(a.out) + at * D + 4 * sub;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) Elem<T>::store(dst + e, m == -INFINITY ? 0.f : acc[e] / l);
+        store4(reinterpret_cast<T*>(a.out) + at * D + 4 * sub, m == -INFINITY ? f32x4_t{0.f, 0.f, 0.f, 0.f} : acc / l);
     }
 }
 
@@ -1053,7 +1062,7 @@ static int check_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
 //      time, and its rows' partial results are written and read once; the number of parts that makes the sum least.
 constexpr int kWantedFew = 2048, kPlaces = 512, kMaxParts = 64;
 struct ListPlan {
-    bool many = false;
+    bool many = false, alone = false;
     int tiles = 1;             // few: tiles a list, many: tiles in all
     int splits = 0;
 };
@@ -1069,6 +1078,8 @@ static ListPlan plan_lists(int64_t lists, int64_t list_rows, int64_t all_rows, i
     if (!p.many) {
         const int64_t most = std::min<int64_t>(kMaxParts, (max_keys + kMinPartFew - 1) / kMinPartFew);
         p.splits = (int)std::max<int64_t>(1, std::min(most, kWantedFew / std::max<int64_t>(lists * hk, 1)));
+        // a wave for a part where four would have a group or two of keys each, once that still leaves every CU a workgroup
+        p.alone = max_keys <= (int64_t)kMinPartFew * p.splits && lists * hk * p.splits >= 1024;
         return p;
     }
     p.tiles = (int)(all_rows / 128 + lists);
@@ -1109,12 +1120,15 @@ static Plan make_plan(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* ba
 
 template <typename T, int D>
 static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists& prefix, const Plan& p, hipStream_t st) {
-    auto blocks_of = [&](const KeyLists& ls) { return (int64_t)a.hk * ls.splits * (ls.many ? ls.tiles : (int64_t)ls.n * ls.tiles); };
+    auto blocks_of = [&](const KeyLists& ls) {
+        const int64_t parts = (int64_t)a.hk * ls.splits * (ls.many ? ls.tiles : (int64_t)ls.n * ls.tiles);
+        return ls.alone ? (parts + 3) / 4 : parts;
+    };
     const int64_t n1 = blocks_of(own);
-    LCM_REQUIRE(n1 <= INT32_MAX / 4, "paged attention: too many rows");
+    LCM_REQUIRE(n1 <= INT32_MAX / 8, "paged attention: too many rows");
     if (prefix.n > 0) {
         const int64_t n0 = blocks_of(prefix);
-        LCM_REQUIRE(n0 <= INT32_MAX / 4, "paged attention: too many rows");
+        LCM_REQUIRE(n0 <= INT32_MAX / 8, "paged attention: too many rows");
         hipLaunchKernelGGL((k_paged_pair<T, D>), dim3((unsigned)((((n0 + 7) >> 3) + ((n1 + 7) >> 3)) << 3)), dim3(256), 0, st, a, prefix, own,
                            (int)n0, (int)n1);
     } else if (own.many) {
@@ -1157,11 +1171,11 @@ static int paged_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     a.g_magic = (uint32_t)((((uint64_t)1 << 32) * ((1u << a.g_shift) - a.G)) / a.G + 1);
     a.scale_log2 = scale * 1.4426950408889634f;
     const KeyLists own{PageTable{batch->page_table, batch->max_pages, page_shift_of(pages), (uint32_t)pages->n_pages}, batch->seq_lens, nullptr,
-                     batch->n_seqs, batch->max_keys, causal != 0, p.own.splits, p.prefix.splits, p.own.many, p.own.tiles};
+                     batch->n_seqs, batch->max_keys, causal != 0, p.own.splits, p.prefix.splits, p.own.many, p.own.tiles, p.own.alone};
     KeyLists pre{};
     if (prefix)
         pre = KeyLists{PageTable{prefix->page_table, prefix->max_pages, page_shift_of(pages), (uint32_t)pages->n_pages}, prefix->lens,
-                            prefix->group_starts, prefix->n_groups, prefix->max_keys, 0, p.prefix.splits, 0, p.prefix.many, p.prefix.tiles};
+                            prefix->group_starts, prefix->n_groups, prefix->max_keys, 0, p.prefix.splits, 0, p.prefix.many, p.prefix.tiles, p.prefix.alone};
     if (p.joined) {
         a.part_ml = reinterpret_cast<float2*>(ws);
         a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + p.ml_bytes);
