@@ -119,7 +119,7 @@ struct Tile16<bf16_t, D> {
     __device__ __forceinline__ void load_v(int h, const bf16_t* base, int lane) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            v[h][e] = *reinterpret_cast<const vpiece_t*>(base + (4 * (lane >> 4) + e) * D + kO * (lane & 15));
+            v[h][e] = __builtin_nontemporal_load(reinterpret_cast<const vpiece_t*>(base + (4 * (lane >> 4) + e) * D + kO * (lane & 15)));
     }
     __device__ __forceinline__ void scores(float (&s)[8]) const {
 #pragma unroll
@@ -209,7 +209,7 @@ struct Tile16<float, D> {
         for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int u = 0; u < D / 64; ++u)
-                v[0][e][u] = *reinterpret_cast<const f32x4_t*>(base + (4 * (lane >> 4) + e) * D + 64 * u + 4 * (lane & 15));
+                v[0][e][u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4_t*>(base + (4 * (lane >> 4) + e) * D + 64 * u + 4 * (lane & 15)));
     }
     __device__ __forceinline__ void scores(float (&s)[4]) const {
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -1060,7 +1060,7 @@ static int check_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
 //      length even out.
 // many: a part takes a workgroup a step for each tile of keys and a few to begin and end, a round of kPlaces workgroups at a
 //      time, and its rows' partial results are written and read once; the number of parts that makes the sum least.
-constexpr int kWantedFew = 2048, kPlaces = 512, kMaxParts = 64;
+constexpr int kWantedFew = 4096, kPlaces = 512, kMaxParts = 64;
 struct ListPlan {
     bool many = false, alone = false;
     int tiles = 1;             // few: tiles a list, many: tiles in all
