@@ -30,13 +30,23 @@ struct HeadArgs {
     int n_seqs, max_keys;
 };
 
-// Eight values as they lie in memory.
+// Eight values as they lie in memory, read past the caches: nobody reads them again (append of 13 thousand rows: 67 -> 60 us).
+// What is written stays in reach of the attention behind.
 template <typename T>
 struct Raw8;
 template <>
-struct Raw8<bf16_t> { uint4 x; };
+struct Raw8<bf16_t> {
+    nv_u4 x;
+    __device__ __forceinline__ void load(const bf16_t* p) { x = __builtin_nontemporal_load(reinterpret_cast<const nv_u4*>(p)); }
+};
 template <>
-struct Raw8<float> { float4 x, y; };
+struct Raw8<float> {
+    nv_u4 x, y;
+    __device__ __forceinline__ void load(const float* p) {
+        x = __builtin_nontemporal_load(reinterpret_cast<const nv_u4*>(p));
+        y = __builtin_nontemporal_load(reinterpret_cast<const nv_u4*>(p) + 1);
+    }
+};
 
 // Value of another lane of the same 16, as an operand modifier of a vector operation (no LDS).
 template <int CTRL>
@@ -173,7 +183,7 @@ __global__ __launch_bounds__(256) void k_head_rows(HeadArgs a, int head_shift, i
 #pragma unroll
             for (int it = 0; it < CHUNK; ++it) {
                 raw[it] = Raw8<T>{};
-                if (h + it * hs < end) raw[it] = *reinterpret_cast<const Raw8<T>*>(from + (h + it * hs - base) * src_head);
+                if (h + it * hs < end) raw[it].load(from + (h + it * hs - base) * src_head);
             }
 #pragma unroll
             for (int it = 0; it < CHUNK; ++it) {

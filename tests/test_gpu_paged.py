@@ -243,7 +243,11 @@ ATTENDS = [
     ([129, 65], [0, 63], 4, 2, 128, 64, True),
     ([300], [5], 5, 5, 128, 128, True),
     ([2, 90], [1500, 3], 32, 8, 128, 256, True),
-    ([17, 16, 15], [15, 16, 17], 3, 1, 64, 16, True)]
+    ([17, 16, 15], [15, 16, 17], 3, 1, 64, 16, True),
+    # more short parts than the chip has places: a wave for each
+    ([1] * 64, [(i * 41) % 256 for i in range(64)], 16, 16, 128, 32, False),
+    ([i % 4 for i in range(128)], [(i * 29) % 200 for i in range(128)], 8, 8, 64, 16, True),
+    ([3] * 65, [0] * 65, 16, 16, 128, 16, True)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
