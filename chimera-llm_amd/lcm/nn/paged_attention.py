@@ -80,15 +80,15 @@ class HeadNorm:
             _hip.require_gpu(t, "head norm weight")
             _require(t.dim() == 1 and t.is_contiguous() and t.shape == given[0].shape and t.dtype == given[0].dtype
                      and t.device == given[0].device, "head norm weights and biases must be alike, contiguous (head_dim,)")
-        self._like = (given[0].shape[0], given[0].dtype, given[0].device) if given else None
+        self._given = given
+        self._head_dim, self._dtype, self._device = (given[0].shape[0], given[0].dtype, given[0].device) if given else (None,) * 3
         self._c = _hip.HeadNorm(*(None if t is None else t.data_ptr() for t in self.tensors), norm_kind(kind), self.eps)
         self._ref = C.byref(self._c)
 
     def _check(self, head_dim: int, dtype: torch.dtype, device: torch.device) -> None:
-        if self._like is not None and self._like != (head_dim, dtype, device):
-            raise ValueError(f"head norm weights are {self._like}, the heads {(head_dim, dtype, device)}")
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in self.tensors):
-            raise RuntimeError(_NO_BACKWARD)
+        if self._given and (self._head_dim != head_dim or self._dtype is not dtype or self._device != device):
+            raise ValueError(f"head norm weights are {(self._head_dim, self._dtype, self._device)}, the heads {(head_dim, dtype, device)}")
+        _grad_free(*self._given)
 
 
 class KVPages:
@@ -191,7 +191,8 @@ def _grad_free(*tensors: Tensor) -> None:
 
 
 def _new(like: Tensor) -> Tensor:
-    return torch.empty_like(like, memory_format=torch.contiguous_format)
+    out = torch.empty_like(like)           # keeps the order of a permuted dense tensor's dimensions
+    return out if out.is_contiguous() else torch.empty(like.shape, dtype=like.dtype, device=like.device)
 
 
 def _heads(t: Tensor, what: str, dtype: torch.dtype, device: torch.device, rows: Optional[int], heads: Optional[int],
