@@ -60,7 +60,7 @@ inline int check_pages(const lcmhip_kv_pages* p) {
 }
 
 inline int check_batch(const lcmhip_kv_pages* p, const lcmhip_paged_batch* b, int64_t rows) {
-    LCM_REQUIRE(b && b->page_table && b->seq_lens, "paged batch: null argument");
+    LCM_REQUIRE(b && (b->n_seqs == 0 || (b->page_table && b->seq_lens)), "paged batch: null argument");
     LCM_REQUIRE(b->n_seqs >= 0 && b->n_seqs <= (1 << 24), "paged batch: n_seqs out of range");
     LCM_REQUIRE(b->max_pages >= 1, "paged batch: max_pages must be positive");
     LCM_REQUIRE(b->max_q >= 1, "paged batch: max_q must be positive");

@@ -1051,7 +1051,7 @@ static int check_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     LCM_TRY(check_batch(pages, batch, rows));
     LCM_REQUIRE(n_heads >= 1 && n_heads <= 65535 && n_heads % pages->n_kv_heads == 0,
                 "paged attention: n_heads must be a multiple of n_kv_heads");
-    LCM_REQUIRE(rows * n_heads <= INT32_MAX, "paged attention: too many rows");
+    LCM_REQUIRE(rows * n_heads <= INT32_MAX - 1024, "paged attention: too many rows");
     return LCMHIP_OK;
 }
 
@@ -1156,7 +1156,7 @@ static int paged_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     LCM_TRY(check_attention(pages, batch, rows, n_heads));
     if (prefix) LCM_TRY(check_prefix(pages, prefix));
     LCM_REQUIRE(q && out, "paged attention: null argument");
-    LCM_REQUIRE(scale > 0.f && scale < INFINITY, "paged attention: scale must be positive and finite");
+    LCM_REQUIRE(scale >= 1e-20f && scale <= 1e20f, "paged attention: scale must lie in [1e-20, 1e20]");
     LCM_TRY(check_rows(q, q_row, q_head, pages->dtype, "paged attention: q"));
     LCM_TRY(check_rows(out, 0, 0, pages->dtype, "paged attention: out"));
     if (rows == 0 || batch->n_seqs == 0) return LCMHIP_OK;

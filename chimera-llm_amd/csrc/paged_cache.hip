@@ -306,7 +306,7 @@ int lcmhip_head_norm_rope(const void* q, int64_t q_row, int64_t q_head, const vo
     a.q_out = q_out; a.qo_row = q_out_row; a.qo_head = q_out_head;
     a.k_out = k_out; a.ko_row = k_out_row; a.ko_head = k_out_head;
     a.rows = rows; a.nq = q ? n_heads : 0; a.nk = k ? n_kv_heads : 0;
-    a.positions = rotary ? positions : nullptr;
+    a.positions = positions;
     return launch_head_rows(a, head_dim, dtype, false, static_cast<hipStream_t>(stream));
 }
 
@@ -325,6 +325,7 @@ int lcmhip_paged_append(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* 
     LCM_TRY(check_rows(q_out, 0, 0, pages->dtype, "paged_append: q_out"));
     HeadArgs a{};
     LCM_TRY(take_transform(a, norm, rotary, pages->head_dim, q != nullptr, true));
+    if (batch->n_seqs == 0) return LCMHIP_OK;              // rows of no sequence
     a.q = q; a.q_row = q_row; a.q_head = q_head; a.k = k; a.k_row = k_row; a.k_head = k_head;
     a.v = v; a.v_row = v_row; a.v_head = v_head;
     a.q_out = q_out; a.qo_head = pages->head_dim; a.qo_row = (int64_t)n_heads * pages->head_dim;

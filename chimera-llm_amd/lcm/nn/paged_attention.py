@@ -133,19 +133,19 @@ class PagedBatch:
         _require(q_starts is not None or max_q == 1, "without q_starts every sequence has one row")
         self.page_table, self.seq_lens, self.q_starts = page_table, seq_lens, q_starts
         self.num_seqs, self.max_pages, self.max_q, self.max_keys = n, page_table.shape[1], int(max_q), max_keys
-        self._c = _hip.PagedBatch(table, lens, starts, n, self.max_pages, self.max_q, 0)
-        self._ref = C.byref(self._c)
-        self._fit = None
+        self._fields, self._refs = (table, lens, starts, n, self.max_pages, self.max_q), {}
 
     def _bind(self, pages: KVPages, rows: int):
-        """The C struct with max_keys filled in for this page size."""
-        if self._fit != pages.page_size:
-            self._c.max_keys, self._fit = _reach(self.max_keys, self.max_pages, pages), pages.page_size
+        """The C struct for this page size."""
         if self.device != pages.device:
             raise ValueError(f"the batch lives on {self.device}, the pages on {pages.device}")
         if self.q_starts is None and rows != self.num_seqs:
             raise ValueError("without q_starts there is one row for every sequence")
-        return self._ref
+        ref = self._refs.get(pages.page_size)
+        if ref is None:
+            ref = C.byref(_hip.PagedBatch(*self._fields, _reach(self.max_keys, self.max_pages, pages)))
+            self._refs[pages.page_size] = ref
+        return ref
 
 
 class SharedPrefix:
@@ -162,16 +162,16 @@ class SharedPrefix:
                  "a shared prefix needs one table row and length for every group and one start more")
         self.page_table, self.lens, self.group_starts = page_table, lens, group_starts
         self.max_pages, self.max_keys = page_table.shape[1], max_keys
-        self._c = _hip.SharedPrefix(table, lens_p, starts, n, self.max_pages, 0)
-        self._ref = C.byref(self._c)
-        self._fit = None
+        self._fields, self._refs = (table, lens_p, starts, n, self.max_pages), {}
 
     def _bind(self, pages: KVPages):
-        if self._fit != pages.page_size:
-            self._c.max_keys, self._fit = _reach(self.max_keys, self.max_pages, pages), pages.page_size
         if self.device != pages.device:
             raise ValueError(f"the prefix lives on {self.device}, the pages on {pages.device}")
-        return self._ref
+        ref = self._refs.get(pages.page_size)
+        if ref is None:
+            ref = C.byref(_hip.SharedPrefix(*self._fields, _reach(self.max_keys, self.max_pages, pages)))
+            self._refs[pages.page_size] = ref
+        return ref
 
 
 def _reach(max_keys: Optional[int], max_pages: int, pages: KVPages) -> int:
@@ -239,8 +239,8 @@ def head_norm_rope(q: Optional[Tensor], k: Optional[Tensor], *, positions: Optio
     """Norm of every query and key head and the position rotation behind it, in one pass: returns (q_out, k_out).
 
     q (rows, heads, head_dim), k (rows, key heads, head_dim), either may be None, may be slices of one stacked product.
-    `positions` (rows,) int32 with `rope`: a row of a negative position is skipped (padding: q_out and k_out keep what they
-    hold there), one beyond the table gives NaN.  q_out / k_out default to new contiguous tensors and may be q / k themselves."""
+    `positions` (rows,) int32, needed with `rope`: a row of a negative position is skipped (padding: q_out and k_out keep what
+    they hold there), one beyond the table gives NaN.  q_out / k_out default to new contiguous tensors and may be q / k themselves."""
     like = q if q is not None else k
     if like is None:
         raise ValueError("head_norm_rope needs queries or keys")
@@ -311,7 +311,7 @@ def paged_append(pages: KVPages, batch: PagedBatch, k: Tensor, v: Tensor, *, q: 
         raise ValueError("q_out without q")
     norm_ref, rope_ref, pos = _transform(rope, norm, positions, k)
     batch_ref = batch._bind(pages, rows)
-    if rows:
+    if rows and batch.num_seqs:            # an empty tensor has no address
         _call(device, _lib.lcmhip_paged_append, pages._ref, batch_ref, *kp, *vp, *qp, qo, rows, heads, norm_ref, rope_ref, pos)
     return q_out
 
@@ -331,7 +331,7 @@ def _attend(q: Tensor, pages: KVPages, batch: PagedBatch, prefix: Optional[Share
     else:
         refs, fn, size_fn = ((pages._ref, batch._bind(pages, rows), prefix._bind(pages)), _lib.lcmhip_shared_prefix_attention,
                              _lib.lcmhip_shared_prefix_attention_workspace)
-    if rows == 0:
+    if rows == 0 or batch.num_seqs == 0:
         return out
     need = C.c_size_t()
     _hip.check(size_fn(*refs, rows, heads, C.byref(need)))
@@ -348,7 +348,7 @@ def paged_attention(q: Tensor, pages: KVPages, batch: PagedBatch, *, causal: boo
     """softmax(scale q K^T) V over the pages of every row's sequence: (rows, heads, head_dim), contiguous.
 
     With `causal` a row sees its sequence up to its own position, otherwise all seq_lens positions.  Query head h reads key head
-    h // (heads // key heads).  `scale` defaults to head_dim ** -0.5 and must be positive.  A row that sees no position gives
+    h // (heads // key heads).  `scale` defaults to head_dim ** -0.5 and must lie in [1e-20, 1e20].  A row that sees no position gives
     zeros; rows of no sequence keep what `out` holds there (undefined without `out`).  `out` must not overlap q."""
     return _attend(q, pages, batch, None, causal, scale, out)
 

@@ -471,8 +471,8 @@ typedef struct {
 
 /* Norm of every query and key head and the rotation behind it in one pass: y = rotate(norm(x)), fp32 inside, rounded once.
  * q, q_out (rows, n_heads, head_dim), k, k_out (rows, n_kv_heads, head_dim) with row / head strides; either pair may be NULL.
- * norm, rotary: NULL for none.  positions (rows) int32, required with rotary: rows of a negative position are skipped (q_out,
- * k_out keep what they hold), a position >= n_positions gives NaN.  q_out may be q and k_out k (same strides). */
+ * norm, rotary: NULL for none.  positions (rows) int32, required with rotary, else optional: rows of a negative position are
+ * skipped (q_out, k_out keep what they hold), a position >= n_positions of a rotation gives NaN.  q_out may be q and k_out k (same strides). */
 int lcmhip_head_norm_rope(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                           void* q_out, int64_t q_out_row, int64_t q_out_head, void* k_out, int64_t k_out_row, int64_t k_out_head,
                           int64_t rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const lcmhip_head_norm* norm,
@@ -490,7 +490,7 @@ int lcmhip_paged_append(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* 
 
 /* softmax(scale q K^T) V over the pages: with causal != 0 row t of sequence b sees the positions [0, seq_lens[b] -
  * (q_starts[b + 1] - t) + 1), otherwise all seq_lens[b].  A row that sees no key gives zeros.  q (rows, n_heads, head_dim)
- * strided, out the same contiguous; scale > 0.  Softmax statistics and sums are fp32.  `workspace` (device, 256-byte aligned) of at
+ * strided, out the same contiguous; scale in [1e-20, 1e20].  Softmax statistics and sums are fp32.  `workspace` (device, 256-byte aligned) of at
  * least lcmhip_paged_attention_workspace bytes holds partial results while the call runs; nothing in it has to be zero and
  * nothing is kept in it between calls, but calls that may overlap must not share one.  bytes == 0: NULL will do. */
 int lcmhip_paged_attention_workspace(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, int64_t rows, int32_t n_heads,

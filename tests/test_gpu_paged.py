@@ -271,6 +271,9 @@ def test_paged_attention(pa, dtype, causal, case):
     batch = pa.PagedBatch(b.table, _int(b.lens), _int(b.starts), max_q=1 + 3 * max(qs))
     again = pa.paged_attention(q[:b.rows], pages, batch, causal=causal, scale=scale)
     _within(again[owned[:b.rows]], want[owned], ref.attend_bound(want, bound, dtype)[owned], case)
+    # a max_q that is too small costs time only
+    again = pa.paged_attention(q[:b.rows], pages, pa.PagedBatch(b.table, _int(b.lens), _int(b.starts), max_q=1), causal=causal, scale=scale)
+    _within(again[owned[:b.rows]], want[owned], ref.attend_bound(want, bound, dtype)[owned], case)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -525,6 +528,39 @@ def test_captured_steps(pa, dtype):
         want = list(step()) + [b.k, b.v]
         for a, e in zip(got, want):
             assert torch.equal(a, e), i
+
+
+def test_empty_batches(pa):
+    """No rows, no sequences, rows of no sequence: nothing is written."""
+    pages = pa.KVPages.create(2, 16, 2, 64, dtype=F32)
+    pages.k.fill_(1.0), pages.v.fill_(2.0)
+    x = torch.ones(3, 2, 64, device="cuda")
+    out = torch.full_like(x, 5.0)
+    none = torch.empty(0, 4, dtype=torch.int32, device="cuda")
+    nobody = pa.PagedBatch(none, _int([]), _int([0]), max_q=1)
+    assert (pa.paged_attention(x, pages, nobody, out=out) == 5).all()
+    assert (pa.paged_append(pages, nobody, x, x, q=x, q_out=out) == 5).all()
+    owned_by_none = pa.PagedBatch(_int([[0]]), _int([4]), _int([0, 0]), max_q=1)
+    assert (pa.paged_attention(x, pages, owned_by_none, out=out) == 5).all()
+    assert (pa.paged_append(pages, owned_by_none, x, x, q=x, q_out=out) == 5).all()
+    prefix = pa.SharedPrefix(_int([[1]]), _int([16]), _int([0, 1]))
+    assert (pa.shared_prefix_attention(x, pages, owned_by_none, prefix, out=out) == 5).all()
+    assert pa.paged_attention(x[:0], pages, pa.PagedBatch(none, _int([]))).shape == (0, 2, 64)
+    assert (pages.k == 1).all() and (pages.v == 2).all()
+
+
+def test_one_batch_over_two_page_sizes(pa):
+    """The bound of the lengths follows the pool that a call names, not the one that was used first."""
+    x = torch.randn(1, 1, 64, device="cuda")
+    batch = pa.PagedBatch(_int([[0]]), _int([40]))
+    outs = []
+    for ps in (16, 64, 16):
+        k = torch.randn(1, 1, ps, 64, device="cuda", generator=_gen(ps))
+        out = pa.paged_attention(x, pa.KVPages(k, k), batch)
+        want, bound, _ = ref.paged(x, k, k, _int([[0]]), [40], None, True, 0.125)
+        _within(out, want, ref.attend_bound(want, bound, F32))
+        outs.append(out)
+    assert torch.equal(outs[0], outs[2])
 
 
 def test_other_streams(pa):

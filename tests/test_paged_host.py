@@ -71,7 +71,7 @@ def test_refused_batches(hip, kw, text):
 @pytest.mark.parametrize("kw,text", [
     (dict(q=None), b"null"), (dict(out=None), b"null"), (dict(q=P + 2), b"16 bytes"), (dict(out=P + 4), b"16 bytes"), (dict(q_row=1025), b"16 bytes"),
     (dict(q_head=132), b"16 bytes"), (dict(rows=-1), b"rows"), (dict(heads=0), b"n_heads"), (dict(heads=5), b"n_heads"),
-    (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale")])
+    (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=1e-30), b"scale"), (dict(scale=1e30), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale")])
 def test_refused_attention_arguments(hip, kw, text):
     _refused(hip, _attend(hip, **kw), text)
     _refused(hip, _attend(hip, prefix=_prefix(hip), **kw), text)
@@ -111,6 +111,14 @@ def test_refused_append(hip):
     for kw, text in [(dict(k=None), b"null"), (dict(v=None), b"null"), (dict(q=P), b"together"), (dict(q_out=P), b"together"),
                      (dict(q=P, q_out=P), b"head count"), (dict(k_row=516), b"16 bytes"), (dict(v=P + 8), b"16 bytes")]:
         _refused(hip, call(**kw), text)
+
+
+def test_no_sequences_is_no_work(hip):
+    """A batch without sequences is accepted with empty arrays, and nothing is launched (there is no GPU here)."""
+    none = _batch(hip, n_seqs=0, page_table=None, seq_lens=None)
+    assert _attend(hip, batch=none) == 0 and _attend(hip, batch=none, prefix=_prefix(hip)) == 0
+    assert hip.lib.lcmhip_paged_append(_pages(hip), none, P, 512, 128, P, 512, 128, None, 0, 0, None, 6, 0, None, None, None, None) == 0
+    assert _attend(hip, batch=_batch(hip, n_seqs=0, q_starts=None), rows=0) == 0
 
 
 def test_workspace_sizes(hip):
