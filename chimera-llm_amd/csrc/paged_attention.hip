@@ -27,7 +27,7 @@ struct KeyLists {
     int n, max_keys;
     int causal;                      // row r of the list sees keys [0, len - rows + r + 1)
     int splits, part0;               // parts of a list, and the number of the first
-    int many, tiles;                 // many_rows(): tiles in all; few_rows(): tiles a list
+    int many, tiles;                 // many_rows(), and how many tiles of rows all lists have together
     int alone;                       // few_rows(): every wave has a part of its own (short parts), or four waves share one
 };
 
@@ -268,7 +268,13 @@ struct Tile16<float, D> {
 };
 
 // Few rows for each list of keys: a tile of 16 (row, head of the group) pairs of one key head against one part of a list, four
-// waves that take the part's groups of keys in turn and join their results in LDS.  Bound by the bytes of the keys and values.
+// waves that take the part's groups of keys in turn and join their results in LDS (or, for short parts, a part for each wave).
+// Bound by the bytes of the keys and values: with one row a list 15 of the 16 columns of a product are empty, and the matrix unit
+// is still busy for less than a third of the time the bytes take.  Two rounds of loads are in flight for every wave (the values of
+// this group, the keys of the next), 128 KB a CU.  One row for each of 64 documents of 1000-3800 keys, 16 heads, bf16: 208 us, 6.3
+// TB/s; two sequences of 120k-131k keys, 8 key heads: 154 us and 5 for the join, 6.2 TB/s; one of 137 keys, fp32: 9 us, of which
+// the chain length -> page -> keys -> values -> join is all.  Eight waves instead of four made that one slower (9.2 against 7.7 us
+// launch to launch).
 template <int D>
 struct FewShared {
     float o[4][16][D + 4];
@@ -283,13 +289,13 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
     const int stride = ls.alone ? Tile::kKeys : 4 * Tile::kKeys;   // from one group of keys of this wave to the next
     if (ls.alone) {
         bid = 4 * bid + wave;
-        if (bid >= a.hk * ls.splits * ls.n * ls.tiles) return;     // no barrier below
+        if (bid >= a.hk * ls.splits * ls.n) return;        // no barrier below
     }
     const int hk = bid % a.hk;
     bid /= a.hk;
     const int split = bid % ls.splits;
     bid /= ls.splits;
-    const int list = bid % ls.n, tile0 = bid / ls.n;
+    const int list = bid;
     const int G = a.G;
     int r0, r1, keys, k0, k1;
     list_extent(a, ls, list, r0, r1, keys);
@@ -298,7 +304,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
     const T* kp = reinterpret_cast<const T*>(a.kp);
     const T* vp = reinterpret_cast<const T*>(a.vp);
 
-    for (int t0 = tile0 * 16; t0 < n_rows; t0 += ls.tiles * 16) {
+    for (int t0 = 0; t0 < n_rows; t0 += 16) {              // more than one tile where a batch's max_q, or its average, said otherwise
         const int mine = t0 + (lane & 15);                 // (row, head) pair of this lane
         const bool live = mine < n_rows;
         const int token = live ? div_g(a, mine) : 0, row = r0 + token;
@@ -699,7 +705,13 @@ __device__ __forceinline__ void lds_dma(const char* base, const uint32_t (&off)[
 
 // Many rows for each list of keys (prompts; all rows of a group against its prefix): a tile of 128 (row, head of the group)
 // pairs of one key head against one part of a list; wave w has pairs 32 w .., and the four share the keys and values that
-// LDS-DMA brings one tile ahead.  Bound by the matrix instructions.
+// LDS-DMA brings one tile ahead.  Two workgroups a CU.
+// Bound by the matrix instructions at the clock that the chip's power leaves them: a stream of them from registers on random data
+// reaches 1500-1700 TFLOP/s in bf16, a large library product 1380, this kernel 1080 on 16384 rows that see 16384 keys, 1020 causal,
+// 900 on eight causal prompts of 1500-2048 rows behind up to 2048 cached positions (450 us), where beginning and ending a
+// workgroup and the tiles on the diagonal count.  Without the LDS-DMA that took 418 of then 470 us, without the exponentials as
+// well 393, with nothing but the products 320.  Measured and left: eight waves that share 256 rows, with two to four buffers (465
+// against 456 us, short prompts 139 against 112), the loop unrolled twice, operands read six or eight products ahead.
 template <typename T, int D>
 struct ManyShared {
     char kv[2][2][Tile32<T, D>::kKeys * Tile32<T, D>::kRow];   // [buffer][keys, values]
@@ -965,7 +977,8 @@ struct JoinArgs {
 };
 
 // Joins the parts of every (row, head).  D / 4 lanes hold a row's values; PG such groups take the parts in turn and meet in LDS
-// (many parts of few rows), or one group takes them all (PG = 1).
+// (many parts of few rows), or one group takes them all (PG = 1).  Latency is all there is to it: 4-5 us a launch where loads
+// depended on the weight of the part before took 39 (64 parts of 64 rows).
 template <typename T, int D, int PG>
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, JoinArgs j) {
     constexpr int L4 = D / 4, ROWS = 256 / L4 / PG, U = 8;
@@ -1055,15 +1068,18 @@ static int check_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
     return LCMHIP_OK;
 }
 
-// How a call is cut.  A list of keys goes to k_paged_few where its rows fill no more than one tile of 16, else to k_paged_many.
-// few: parts are added until the grid has kWantedFew workgroups, four for each place on the chip, so that lists of unequal
-//      length even out.
-// many: a part takes a workgroup a step for each tile of keys and a few to begin and end, a round of kPlaces workgroups at a
-//      time, and its rows' partial results are written and read once; the number of parts that makes the sum least.
+// How a call is cut.  A list of keys goes to few_rows() where its rows fill no more than one tile of 16, else to many_rows(): 64
+// lists of 2048 keys with 16 rows a key head take 104 / 98 us (few / many, bf16) and 211 / 301 us (fp32), with 32 rows 189 / 99 us
+// and 387 / 292 us.
+// few: parts are added until the grid has kWantedFew workgroups, eight for each place on the chip, so that lists of unequal
+//      length even out (64 lists of 1000-3800 keys: 238 us with 2048 workgroups, 231 with 4096 or 8192).
+// many: a part takes a workgroup a step for each tile of keys and 3 us to begin and end, a round of kPlaces workgroups at a time,
+//      and its rows' partial results are written and read once (about 3 TB/s); the number of parts that makes the sum least.
+//      Twelve parts of a prefix of 3701 positions for 64 rows: 31.7 us, 4 parts 38.3, 32 parts 34.7.
 constexpr int kWantedFew = 4096, kPlaces = 512, kMaxParts = 64;
 struct ListPlan {
     bool many = false, alone = false;
-    int tiles = 1;             // few: tiles a list, many: tiles in all
+    int tiles = 0;             // many: tiles of rows in all
     int splits = 0;
 };
 struct Plan {
@@ -1086,7 +1102,7 @@ static ListPlan plan_lists(int64_t lists, int64_t list_rows, int64_t all_rows, i
     // workgroups of one part, if the lists have about as many rows each
     const int64_t blocks = hk * std::max((all_rows + 127) / 128, lists * ((all_rows / lists + 127) / 128));
     const int step_keys = dtype == LCMHIP_BF16 ? 64 : 32;
-    const double step_us = (dtype == LCMHIP_BF16 ? 0.9 : 6.8) * head_dim / 128;
+    const double step_us = (dtype == LCMHIP_BF16 ? 0.9 : 6.8) * head_dim / 128;   // two workgroups a CU at the matrix unit's rate
     const double join_us = (double)all_rows * hk * head_dim * 8 / 3e6;
     const int most = std::min(kMaxParts, (max_keys + 2 * step_keys - 1) / (2 * step_keys));
     double best = 0;
@@ -1121,7 +1137,7 @@ static Plan make_plan(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* ba
 template <typename T, int D>
 static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists& prefix, const Plan& p, hipStream_t st) {
     auto blocks_of = [&](const KeyLists& ls) {
-        const int64_t parts = (int64_t)a.hk * ls.splits * (ls.many ? ls.tiles : (int64_t)ls.n * ls.tiles);
+        const int64_t parts = (int64_t)a.hk * ls.splits * (ls.many ? ls.tiles : ls.n);
         return ls.alone ? (parts + 3) / 4 : parts;
     };
     const int64_t n1 = blocks_of(own);

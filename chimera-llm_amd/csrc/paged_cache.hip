@@ -7,6 +7,10 @@
 //     rotation  (y_i, y_j) -> (y_i cos - y_j sin, y_i sin + y_j cos), j = i + 1 or i + rotary_dim / 2
 // in fp32, rounded once when it is stored.  The sums run over the D / 8 lanes of a head; the partner of a pair (i, i + 1) is
 // in the same lane, that of (i, i + rotary_dim / 2) rotary_dim / 16 lanes away.
+//
+// Bound by bytes read and written, each once: 16384 rows of 32 + 8 heads of 128, bf16, in 65 us (5.3 TB/s; a large copy reaches 5.0),
+// 13 thousand rows of 32 + 8 + 8 heads appended behind ragged histories in 65 us (5.1 TB/s); 64 rows in 3.6 us, a launch.  A head at
+// a time, with its angles and its place looked up for each, took 96 and 127 us: 220 vector operations a kilobyte.
 #include <algorithm>
 
 #include "paged.h"
