@@ -693,14 +693,19 @@ struct Tile32<float, D> {
 // 64 lanes bring 16 bytes each, from base + off[j] + 1024 j (base the same for the wave) to the 1024 bytes at LDS offset dst +
 // 1024 j, for j < N.  Written in assembly because the compiler waits for every outstanding LDS-DMA before any LDS read, whatever
 // it reads; nothing is returned in registers, and the waits for the data are the loop's own (s_waitcnt vmcnt before the
-// barrier).  M0 holds nothing across instructions of the compiler.
+// barrier).  One block for all of them: M0, which says where in LDS they go, is set and used in it.
 template <int N>
 __device__ __forceinline__ void lds_dma(const char* base, const uint32_t (&off)[N], uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off[0]), "s"(base) : "memory");
-    if constexpr (N > 1) asm volatile("global_load_lds_dwordx4 %0, %1 offset:1024" ::"v"(off[1]), "s"(base) : "memory");
-    if constexpr (N > 2) asm volatile("global_load_lds_dwordx4 %0, %1 offset:2048" ::"v"(off[2]), "s"(base) : "memory");
-    if constexpr (N > 3) asm volatile("global_load_lds_dwordx4 %0, %1 offset:3072" ::"v"(off[3]), "s"(base) : "memory");
-    static_assert(N <= 4, "offsets are 12 bits");
+    static_assert(N == 1 || N == 2 || N == 4, "offsets are 12 bits");
+    if constexpr (N == 1)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off[0]), "s"(base) : "memory", "m0");
+    if constexpr (N == 2)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(dst),
+                     "v"(off[0]), "v"(off[1]), "s"(base) : "memory", "m0");
+    if constexpr (N == 4)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %3, %5 offset:2*1024\n\tglobal_load_lds_dwordx4 %4, %5 offset:3*1024" ::"s"(dst),
+                     "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory", "m0");
 }
 
 // Many rows for each list of keys (prompts; all rows of a group against its prefix): a tile of 128 (row, head of the group)
