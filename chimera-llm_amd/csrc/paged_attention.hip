@@ -25,7 +25,7 @@ struct KeyLists {
     const int32_t* lens;
     const int32_t* group_starts;     // null: list i belongs to sequence i
     int n, max_keys;
-    int causal;                      // row r of the list sees keys [0, len - rows + r + 1)
+    int causal;                      // row r of the list sees keys [0, len - rows + r + 1), of those that are there
     int splits, part0;               // parts of a list, and the number of the first
     int many, tiles;                 // many_rows(), and how many tiles of rows all lists have together
     int alone;                       // few_rows(): every wave has a part of its own (short parts), or four waves share one
@@ -47,8 +47,9 @@ struct PagedArgs {
 
 __device__ __forceinline__ int div_g(const PagedArgs& a, int x) { return (int)((__umulhi(a.g_magic, (uint32_t)x) + (uint32_t)x) >> a.g_shift); }
 
-// Rows and keys of list i.
-__device__ __forceinline__ void list_extent(const PagedArgs& a, const KeyLists& ls, int i, int& r0, int& r1, int& keys) {
+// Rows of list i, its length and how many of its keys are there.  Rows are counted back from the length: a list that is longer
+// than max_keys ends in rows whose own positions are not there and which see all keys.
+__device__ __forceinline__ void list_extent(const PagedArgs& a, const KeyLists& ls, int i, int& r0, int& r1, int& len, int& keys) {
     int s0 = i, s1 = i + 1;
     if (ls.group_starts) {
         s0 = min(max(read_index(ls.group_starts + i), 0), a.n_seqs);
@@ -58,7 +59,8 @@ __device__ __forceinline__ void list_extent(const PagedArgs& a, const KeyLists& 
     r1 = a.q_starts ? read_index(a.q_starts + s1) : s1;
     r0 = min(max(r0, 0), a.rows);
     r1 = min(max(r1, r0), a.rows);
-    keys = max(0, min(read_index(ls.lens + i), ls.max_keys));
+    len = max(0, read_index(ls.lens + i));
+    keys = min(len, ls.max_keys);
 }
 
 constexpr int kMinPartFew = 256;   // keys a workgroup of k_paged_few is worth
@@ -297,8 +299,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
     bid /= ls.splits;
     const int list = bid;
     const int G = a.G;
-    int r0, r1, keys, k0, k1;
-    list_extent(a, ls, list, r0, r1, keys);
+    int r0, r1, len, keys, k0, k1;
+    list_extent(a, ls, list, r0, r1, len, keys);
     part_range<32>(keys, ls.splits, kMinPartFew, split, k0, k1);
     const int n_rows = (r1 - r0) * G;
     const T* kp = reinterpret_cast<const T*>(a.kp);
@@ -310,9 +312,9 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, const KeyLists& ls,
         const int token = live ? div_g(a, mine) : 0, row = r0 + token;
         const int head = hk * G + (live ? mine - token * G : 0);
         // keys that this row and the tile's first row see (later rows see no fewer)
-        const int limit = ls.causal ? keys - (r1 - row) + 1 : keys;
-        const int first_limit = ls.causal ? keys - (r1 - r0 - div_g(a, t0)) + 1 : keys;
-        const int last_limit = ls.causal ? keys - (r1 - r0 - div_g(a, min(t0 + 15, n_rows - 1))) + 1 : keys;
+        const int limit = ls.causal ? len - (r1 - row) + 1 : keys;
+        const int first_limit = ls.causal ? len - (r1 - r0 - div_g(a, t0)) + 1 : keys;
+        const int last_limit = ls.causal ? len - (r1 - r0 - div_g(a, min(t0 + 15, n_rows - 1))) + 1 : keys;
         const int end = min(k1, last_limit);
 
         Tile t;
@@ -737,17 +739,18 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const KeyLists& ls
     // Late tiles first: under a causal mask they have the most keys.
     const int tile = ls.tiles - 1 - bid / ls.splits;
     // 64 lists at a time, a lane each; the first whose tiles do not end before this one
-    int list = -1, r0 = 0, r1 = 0, keys = 0, k0, k1;
+    int list = -1, r0 = 0, r1 = 0, len = 0, keys = 0, k0, k1;
     for (int first = 0; first < ls.n; first += 64) {
-        int x0 = 0, x1 = 0, xk = 0;
+        int x0 = 0, x1 = 0, xl = 0, xk = 0;
         const bool is_list = first + lane < ls.n;
-        if (is_list) list_extent(a, ls, first + lane, x0, x1, xk);
+        if (is_list) list_extent(a, ls, first + lane, x0, x1, xl, xk);
         const int c = __popcll(__ballot(is_list && (int)((int64_t)x1 * G >> 7) + first + lane + 1 <= tile));
         if (c < min(64, ls.n - first)) {
             list = first + c;
             r0 = __builtin_amdgcn_readlane(x0, c);
             r1 = __builtin_amdgcn_readlane(x1, c);
-            keys = __builtin_amdgcn_readlane(xk, c);
+            len = __builtin_amdgcn_readlane(xl, c);
+            keys = min(len, ls.max_keys);
             break;
         }
     }
@@ -761,12 +764,12 @@ __device__ __forceinline__ void many_rows(const PagedArgs& a, const KeyLists& ls
     const bool live = mine < n_rows;
     const int token = live ? div_g(a, mine) : 0, row = r0 + token;
     const int head = hk * G + (live ? mine - token * G : 0);
-    const int at_end = keys - (r1 - r0) + 1;               // keys that the list's first row sees
-    const int limit = ls.causal ? keys - (r1 - row) + 1 : keys;
+    const int at_end = len - (r1 - r0) + 1;                // keys that the list's first row sees, if they are there
+    const int limit = ls.causal ? len - (r1 - row) + 1 : keys;
     const int tile_end = min(k1, ls.causal ? at_end + div_g(a, min(t0 + 127, n_rows - 1)) : keys);
     const int tile_first = ls.causal ? at_end + div_g(a, t0) : keys;
     const bool wave_live = t0 + 32 * wave < n_rows;
-    const int wave_first = ls.causal ? at_end + div_g(a, t0 + 32 * wave) : keys;
+    const int wave_first = ls.causal ? at_end + div_g(a, min(t0 + 32 * wave, n_rows - 1)) : keys;
     const int wave_end = !wave_live ? 0 : min(k1, ls.causal ? at_end + div_g(a, min(t0 + 32 * wave + 31, n_rows - 1)) : keys);
 
     Tile t;

@@ -94,10 +94,13 @@ __global__ __launch_bounds__(256) void k_head_rows(HeadArgs a, int head_shift, i
         const int b = owned ? seq : 0;
         int64_t r0, r1;
         seq_rows(a.q_starts, b, a.rows, r0, r1);
-        const int len = max(0, min(a.seq_lens[b], a.max_keys));
-        const int c = (int)max((int64_t)-1, len - (r1 - row));
+        // counted back from the length as it is: a position from max_keys on has no place, and cutting the length first would
+        // move its row onto a position that is there
+        const int64_t at = a.seq_lens[b] - (r1 - row);
+        const bool placed = at >= 0 && at < a.max_keys;
+        const int c = placed ? (int)at : 0;
         pos = a.positions ? a.positions[row] : c;
-        live = owned && row >= r0 && c >= 0 && pos >= 0;
+        live = owned && row >= r0 && placed && pos >= 0;
         page = a.table.page(b, live ? c : 0);
         in_pool = ((((size_t)max(page, 0) * a.nk) << a.table.page_shift) + (c & ((1 << a.table.page_shift) - 1))) * D + i0;
     } else {

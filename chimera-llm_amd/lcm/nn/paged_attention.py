@@ -116,7 +116,8 @@ class PagedBatch:
     """The sequences of one step.  Sequence b owns the rows [q_starts[b], q_starts[b + 1]) of the q / k / v tensors (q_starts None:
     row b), its newest positions; seq_lens[b] counts its positions including them, and position c lies in page
     page_table[b, c // page_size].  `max_q` is the most rows of one sequence, `max_keys` an upper bound of seq_lens (None: what
-    the table can hold); both choose how the work is split, and lengths are cut to max_keys."""
+    the table can hold); both choose how the work is split.  Positions from max_keys on are not there: a row of such a position is
+    not stored, and no row sees one."""
 
     def __init__(self, page_table: Tensor, seq_lens: Tensor, q_starts: Optional[Tensor] = None, max_q: int = 1,
                  max_keys: Optional[int] = None) -> None:
@@ -290,8 +291,8 @@ def paged_append(pages: KVPages, batch: PagedBatch, k: Tensor, v: Tensor, *, q: 
 
     k, v (rows, key heads, head_dim), q (rows, heads, head_dim), strided.  Row t of sequence b becomes position
     seq_lens[b] - (q_starts[b + 1] - t) of the sequence and is rotated by positions[t] (int32), or by that position when
-    `positions` is None.  Rows without a place (before the sequence's beginning, behind its table, of no sequence, or of a
-    negative position) are skipped."""
+    `positions` is None.  Rows without a place (before the sequence's beginning, from the batch's max_keys on, of no sequence, or of a
+    negative position) are skipped: nothing is stored, and q_out keeps what it holds there (undefined without `q_out`)."""
     _grad_free(k, v)
     dtype, device, head_dim, kv_heads = pages.dtype, pages.device, pages.head_dim, pages.num_kv_heads
     kp = _heads(k, "k", dtype, device, None, kv_heads, head_dim)

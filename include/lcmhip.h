@@ -412,7 +412,8 @@ int lcmhip_attention(const void* q, const void* k_cache, const void* v_cache, co
  * All index arrays are int32 DEVICE arrays that the kernels read when they run (so a captured graph may be replayed on new
  * contents); the host numbers of the structs are bounds.  What the arrays say is never trusted with an address:
  *  - a page id outside [0, n_pages) names a page that is not there: nothing is stored to it and its keys are left out;
- *  - sequence lengths are cut to [0, min(max_keys, max_pages * page_size)], row ranges to [0, rows];
+ *  - positions from max_keys on are not there, however long a sequence says it is: nothing is stored at them and no row sees them
+ *    (a sequence's rows keep their positions, counted back from its length); a negative length is 0; row ranges are cut to [0, rows];
  *  - rows that belong to no sequence (before q_starts[0], from q_starts[n_seqs] on) are neither read nor written.
  * Row pointers are 16-byte aligned and their strides (in elements) a multiple of 16 bytes; the last dimension is dense.
  * head_dim is 64 or 128, page_size a power of two from 16 to 65536, n_heads a multiple of n_kv_heads (query head h reads key head
@@ -481,7 +482,7 @@ int lcmhip_head_norm_rope(const void* q, int64_t q_row, int64_t q_head, const vo
 /* Stores the batch's rows of k (normed and rotated as above) and v into the pages of their sequences; q (NULL: none) goes
  * through the same norm and rotation into q_out, contiguous (rows, n_heads, head_dim), in the same pass.  Row t of sequence b has
  * cache position c = seq_lens[b] - (q_starts[b + 1] - t); it is rotated by positions[t], or by c when positions is NULL.  Rows
- * with c < 0, c beyond the table or a negative position are skipped.  Two sequences that name the same page write it both.
+ * with c < 0, c >= max_keys or a negative position are skipped (q_out keeps what it holds).  Two sequences that name the same page write it both.
  * rows: the rows that q, k and v hold. */
 int lcmhip_paged_append(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* batch, const void* k, int64_t k_row, int64_t k_head,
                         const void* v, int64_t v_row, int64_t v_head, const void* q, int64_t q_row, int64_t q_head, void* q_out,
@@ -489,7 +490,7 @@ int lcmhip_paged_append(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* 
                         const int32_t* positions, void* stream);
 
 /* softmax(scale q K^T) V over the pages: with causal != 0 row t of sequence b sees the positions [0, seq_lens[b] -
- * (q_starts[b + 1] - t) + 1), otherwise all seq_lens[b].  A row that sees no key gives zeros.  q (rows, n_heads, head_dim)
+ * (q_starts[b + 1] - t) + 1), otherwise all seq_lens[b]; of either those below max_keys.  A row that sees no key gives zeros.  q (rows, n_heads, head_dim)
  * strided, out the same contiguous; scale in [1e-20, 1e20].  Softmax statistics and sums are fp32.  `workspace` (device, 256-byte aligned) of at
  * least lcmhip_paged_attention_workspace bytes holds partial results while the call runs; nothing in it has to be zero and
  * nothing is kept in it between calls, but calls that may overlap must not share one.  bytes == 0: NULL will do. */

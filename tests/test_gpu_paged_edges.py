@@ -1,0 +1,130 @@
+"""Calls at the edges of what the paged cache operators (lcm.nn.paged_attention) document, against plain 64-bit statements."""
+
+import pytest
+import torch
+
+from tests import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def pa():
+    assert torch.cuda.is_available()
+    from lcm.nn import paged_attention
+    return paged_attention
+
+
+def _randn(g, *shape, dtype=F32, gain=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * gain).to(dtype)
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _int(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _within(got, want, bound, what=""):
+    assert torch.isfinite(got).all(), what
+    over = (got.double() - want).abs() - bound
+    i = int(over.argmax())
+    assert float(over.max()) <= 0, (what, i, float(got.flatten()[i]), float(want.flatten()[i]), float(bound.flatten()[i]))
+
+
+# ---- sequences longer than the cache can hold ---------------------------------------------------------------------------
+def _overlong(pa, g, dtype, qs, lens, pages_each, ps, hk, d, max_keys):
+    n, rows = len(qs), sum(qs)
+    k, v = _randn(g, n * pages_each, hk, ps, d, dtype=dtype), _randn(g, n * pages_each, hk, ps, d, dtype=dtype)
+    table = torch.randperm(n * pages_each, generator=g, device="cuda").to(torch.int32).view(n, pages_each)
+    starts = [sum(qs[:i]) for i in range(n + 1)]
+    batch = pa.PagedBatch(table, _int(lens), _int(starts), max_q=max(qs), max_keys=max_keys)
+    bound = pages_each * ps if max_keys is None else max_keys
+    return pa.KVPages(k, v), batch, table, starts, rows, bound
+
+
+OVERLONG = [
+    # qs, lens, pages of a sequence, page size, max_keys
+    ([1, 1, 1], [16, 17, 2**31 - 1], 1, 16, None),
+    ([4, 4, 4, 4], [18, 20, 24, 21], 4, 16, 20),             # the table has room behind max_keys
+    ([3, 150, 70], [2**31 - 1, 140, 200], 4, 32, 127),
+    ([2, 3], [300, 33], 2, 16, 31)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("case", range(len(OVERLONG)))
+def test_positions_past_the_bound_are_not_there(pa, dtype, case):
+    """Row t of a sequence is position len - (end - t) however long the sequence is; a position from max_keys on has no place:
+    nothing is stored over the positions before it, its row is skipped, and rows see the keys below max_keys only."""
+    qs, lens, each, ps, max_keys = OVERLONG[case]
+    g = _gen(300 + case)
+    hq, hk, d = 4, 2, 64
+    pages, batch, table, starts, rows, bound = _overlong(pa, g, dtype, qs, lens, each, ps, hk, d, max_keys)
+    rope = pa.RotaryTable.create(256, d)
+    x = _randn(g, rows, hq + 2 * hk, d, dtype=dtype)
+    q_out = torch.full((rows, hq, d), 3.0, dtype=dtype, device="cuda")
+    want_k, want_v = pages.k.double(), pages.v.double()
+    bound_k = torch.zeros_like(want_k)
+    at = [lens[b] - (starts[b + 1] - t) for b in range(len(qs)) for t in range(starts[b], starts[b + 1])]
+    seq = [b for b, n in enumerate(qs) for _ in range(n)]
+    stored = [t for t in range(rows) if 0 <= at[t] < bound]
+    pos = _int([max(0, min(c, 255)) for c in at])
+    y, slack = ref.heads(x[:, hq:hq + hk], None, None, None, 0, rope.cos, rope.sin, "pairs", pos)
+    for t in stored:
+        page, off = int(table[seq[t], at[t] // ps]), at[t] % ps
+        want_k[page, :, off], want_v[page, :, off] = y[t], x[t, hq + hk:].double()
+        bound_k[page, :, off] = ref.heads_bound(y[t], slack[t], dtype)
+    pa.paged_append(pages, batch, x[:, hq:hq + hk], x[:, hq + hk:], q=x[:, :hq], rope=rope, q_out=q_out)
+    _within(pages.k, want_k, bound_k, "keys")
+    assert torch.equal(pages.v.double(), want_v)
+    y, slack = ref.heads(x[:, :hq], None, None, None, 0, rope.cos, rope.sin, "pairs", pos)
+    skipped = [t for t in range(rows) if t not in stored]
+    assert (q_out[skipped] == 3).all()
+    _within(q_out[stored], y[stored], ref.heads_bound(y, slack, dtype)[stored], "queries")
+    # what the rows see: positions up to their own, and none from the bound on
+    q = x[:, :hq].contiguous()
+    for causal in (True, False):
+        out = pa.paged_attention(q, pages, batch, causal=causal)
+        for b in range(len(qs)):
+            r = slice(starts[b], starts[b + 1])
+            keys = min(lens[b], bound)
+            kk, there = ref.gather(pages.k, table[b], keys, ps)
+            vv, _ = ref.gather(pages.v, table[b], keys, ps)
+            visible = torch.tensor([max(0, min(c + 1, keys)) if causal else keys for c in at[r]], device="cuda")
+            want, slack = ref.attend(q[r], kk, vv, there, visible, d ** -0.5)
+            _within(out[r], want, ref.attend_bound(want, slack, dtype), (causal, b))
+
+
+def test_bad_places_are_skipped(pa):
+    """Bad page ids, rows before a sequence's beginning and behind its table, negative positions, starts that lie outside the rows:
+    nothing else is written."""
+    g = _gen(1)
+    ps, hk, d = 16, 2, 64
+    k_pages = torch.full((4, hk, ps, d), 5.0, device="cuda")
+    v_pages = torch.full_like(k_pages, 6.0)
+    pages = pa.KVPages(k_pages, v_pages)
+    table = _int([[0, 4], [-1, 1], [2**31 - 1, -2**31], [2, 3]])
+    lens, starts = _int([18, 3, 5, 2]), _int([0, 3, 5, 6, 9])
+    x = _randn(g, 12, hk, d)
+    q_out = torch.full((12, hk, d), 8.0, device="cuda")
+    pos = _int([0] * 8 + [-1] + [0] * 3)
+    pa.paged_append(pages, pa.PagedBatch(table, lens, starts, max_q=3), x, x, q=x, positions=pos, q_out=q_out)
+    want_k, want_v = torch.full_like(k_pages, 5.0), torch.full_like(v_pages, 6.0)
+    want_k[0, :, 15] = want_v[0, :, 15] = x[0]
+    want_k[2, :, 0] = want_v[2, :, 0] = x[7]
+    assert torch.equal(k_pages, want_k) and torch.equal(v_pages, want_v)
+    assert torch.equal(q_out[:6], x[:6]) and torch.equal(q_out[7], x[7]) and (q_out[[6, 8, 9, 10, 11]] == 8).all()
+    # a length far behind the table and a negative one, starts outside the rows: no row has a place
+    k_pages.fill_(5.0), v_pages.fill_(6.0)
+    pa.paged_append(pages, pa.PagedBatch(_int([[0], [1]]), _int([2**31 - 1, -7]), _int([-3, 2, 2**31 - 1]), max_q=3), x, x)
+    assert (k_pages == 5).all() and (v_pages == 6).all()
+    # the same starts, with a length that gives the first range its places: its two rows that exist are the positions 14 and 15
+    pa.paged_append(pages, pa.PagedBatch(_int([[0], [1]]), _int([16, -7]), _int([-3, 2, 2**31 - 1]), max_q=3), x, x)
+    assert torch.equal(k_pages[0, :, 14:16].transpose(0, 1), x[:2]) and torch.equal(v_pages[0, :, 14:16].transpose(0, 1), x[:2])
+    assert (k_pages[0, :, :14] == 5).all() and (k_pages[1:] == 5).all() and (v_pages[1:] == 6).all()
