@@ -11,7 +11,8 @@ and between a layer's q / k / v products and its output product stand
 `pages` differ from layer to layer, `batch` (and `SharedPrefix`) is made once for a step and used by every layer.
 
 All of it runs on the HIP library only (float32 and bfloat16, head widths 64 and 128) and on the current stream of the
-tensors' device.  There is no backward: inputs that require a gradient are refused while gradients are recorded.  Index tensors
+tensors' device.  There is no derivative: a tensor of a call (inputs, pages, norm weights, rotary
+tables, given outputs) that requires a gradient while gradients are recorded, or that carries a forward-mode tangent, is refused.  Index tensors
 (page tables, lengths, row starts, positions) are int32 tensors on the same device which the kernels read when they run; a
 captured graph can be replayed on new contents of the same tensors.  What they hold is not checked on the host (that would
 wait for the GPU), but it cannot make a kernel leave its buffers: see include/lcmhip.h for what a wrong entry does.
@@ -22,12 +23,14 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from lcm import _hip
 from lcm.nn.normalization import norm_kind
 
 _lib = _hip.lib
 _NO_BACKWARD = "the paged cache operators have no backward: call them under torch.no_grad() or detach the inputs"
+_NO_TANGENT = "the paged cache operators have no forward-mode derivative: detach the inputs"
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -184,11 +187,15 @@ def _reach(max_keys: Optional[int], max_pages: int, pages: KVPages) -> int:
     return max_keys
 
 
-def _grad_free(*tensors: Tensor) -> None:
+def _grad_free(*tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
-            if t.requires_grad:
+            if t is not None and t.requires_grad:
                 raise RuntimeError(_NO_BACKWARD)
+    if forward_ad._current_level >= 0:     # inside forward_ad.dual_level(); torch.no_grad() does not end it
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(_NO_TANGENT)
 
 
 def _new(like: Tensor) -> Tensor:
@@ -225,8 +232,10 @@ def _transform(rope: Optional[RotaryTable], norm: Optional[HeadNorm], positions:
     device = like.device
     if norm is not None:
         norm._check(head_dim, like.dtype, device)
-    if rope is not None and rope.device != device:
-        raise ValueError(f"the rotary table lives on {rope.device}, not on {device}")
+    if rope is not None:
+        _grad_free(rope.cos, rope.sin)
+        if rope.device != device:
+            raise ValueError(f"the rotary table lives on {rope.device}, not on {device}")
     pos = None
     if positions is not None:
         if positions.dtype is not torch.int32 or positions.shape != (rows,) or positions.device != device or not positions.is_contiguous():
@@ -251,10 +260,10 @@ def head_norm_rope(q: Optional[Tensor], k: Optional[Tensor], *, positions: Optio
     if not like.is_cuda:
         _hip.require_gpu(like, "heads")
     rows, _, head_dim = shape
+    _grad_free(q, k, q_out, k_out)
     q_args = k_args = qo_args = ko_args = (None, 0, 0)
     q_heads = k_heads = 0
     if q is not None:
-        _grad_free(q)
         q_args, q_heads = _heads(q, "q", dtype, device, rows, None, head_dim), shape[1]
         if q_out is None:
             q_out = _new(q)
@@ -264,7 +273,6 @@ def head_norm_rope(q: Optional[Tensor], k: Optional[Tensor], *, positions: Optio
     elif q_out is not None:
         raise ValueError("q_out without q")
     if k is not None:
-        _grad_free(k)
         k_args, k_heads = _heads(k, "k", dtype, device, rows, None, head_dim), k.shape[1]
         if k_out is None:
             k_out = _new(k)
@@ -293,14 +301,13 @@ def paged_append(pages: KVPages, batch: PagedBatch, k: Tensor, v: Tensor, *, q: 
     seq_lens[b] - (q_starts[b + 1] - t) of the sequence and is rotated by positions[t] (int32), or by that position when
     `positions` is None.  Rows without a place (before the sequence's beginning, from the batch's max_keys on, of no sequence, or of a
     negative position) are skipped: nothing is stored, and q_out keeps what it holds there (undefined without `q_out`)."""
-    _grad_free(k, v)
+    _grad_free(k, v, q, q_out, pages.k, pages.v)
     dtype, device, head_dim, kv_heads = pages.dtype, pages.device, pages.head_dim, pages.num_kv_heads
     kp = _heads(k, "k", dtype, device, None, kv_heads, head_dim)
     rows = k.shape[0]
     vp = _heads(v, "v", dtype, device, rows, kv_heads, head_dim)
     qp, heads, qo = (None, 0, 0), 0, None
     if q is not None:
-        _grad_free(q)
         qp, heads = _heads(q, "q", dtype, device, rows, None, head_dim), q.shape[1]
         if q_out is None:
             q_out = _new(q)
@@ -319,7 +326,7 @@ def paged_append(pages: KVPages, batch: PagedBatch, k: Tensor, v: Tensor, *, q: 
 
 def _attend(q: Tensor, pages: KVPages, batch: PagedBatch, prefix: Optional[SharedPrefix], causal: bool, scale: Optional[float],
             out: Optional[Tensor]) -> Tensor:
-    _grad_free(q)
+    _grad_free(q, out, pages.k, pages.v)
     qp = _heads(q, "q", pages.dtype, pages.device, None, None, pages.head_dim)
     rows, heads, head_dim = q.shape
     if out is None:

@@ -128,3 +128,58 @@ def test_bad_places_are_skipped(pa):
     pa.paged_append(pages, pa.PagedBatch(_int([[0], [1]]), _int([16, -7]), _int([-3, 2, 2**31 - 1]), max_q=3), x, x)
     assert torch.equal(k_pages[0, :, 14:16].transpose(0, 1), x[:2]) and torch.equal(v_pages[0, :, 14:16].transpose(0, 1), x[:2])
     assert (k_pages[0, :, :14] == 5).all() and (k_pages[1:] == 5).all() and (v_pages[1:] == 6).all()
+
+
+# ---- derivatives -------------------------------------------------------------------------------------------------------------
+def test_every_tensor_of_a_call_is_refused_with_a_gradient_or_a_tangent(pa):
+    """Nothing that a derivative would flow through is used without one: inputs, pages, norm weights and biases, rotary tables and
+    outputs that the caller gives."""
+    n, hq, hk, d, ps = 3, 4, 2, 64, 16
+    g = _gen(17)
+
+    def made(name, change):
+        """The four calls on fresh tensors, the one called `name` passed through `change`."""
+        t = dict(q=_randn(g, n, hq, d), k=_randn(g, n, hk, d), v=_randn(g, n, hk, d), k_pages=_randn(g, 4, hk, ps, d), v_pages=_randn(g, 4, hk, ps, d),
+                 qw=torch.ones(d, device="cuda"), kw=torch.ones(d, device="cuda"), qb=torch.zeros(d, device="cuda"), kb=torch.zeros(d, device="cuda"),
+                 cos=torch.ones(64, d // 2, device="cuda"), sin=torch.zeros(64, d // 2, device="cuda"), q_out=torch.zeros(n, hq, d, device="cuda"),
+                 k_out=torch.zeros(n, hk, d, device="cuda"))
+        if name:
+            t[name] = change(t[name])
+        pages = pa.KVPages(t["k_pages"], t["v_pages"])
+        batch = pa.PagedBatch(_int([[0], [1], [2]]), _int([5, 6, 7]))
+        prefix = pa.SharedPrefix(_int([[3]]), _int([9]), _int([0, 3]))
+        how = dict(rope=pa.RotaryTable(t["cos"], t["sin"]), norm=pa.HeadNorm("standard", t["qw"], t["kw"], t["qb"], t["kb"]))
+        pos = _int([4, 5, 6])
+        heads, store = ["cos", "sin", "qw", "kw", "qb", "kb", "q", "k", "q_out"], ["k_pages", "v_pages", "v"]
+        return [(heads + ["k_out"], lambda: pa.head_norm_rope(t["q"], t["k"], positions=pos, q_out=t["q_out"], k_out=t["k_out"], **how)),
+                (heads + store, lambda: pa.paged_append(pages, batch, t["k"], t["v"], q=t["q"], q_out=t["q_out"], **how)),
+                (["q", "q_out", "k_pages", "v_pages"], lambda: pa.paged_attention(t["q"], pages, batch, out=t["q_out"])),
+                (["q", "q_out", "k_pages", "v_pages"], lambda: pa.shared_prefix_attention(t["q"], pages, batch, prefix, out=t["q_out"]))]
+
+    for _, call in made(None, None):
+        call()
+    names = ["q", "k", "v", "k_pages", "v_pages", "qw", "kw", "qb", "kb", "cos", "sin", "q_out", "k_out"]
+    for name in names:
+        for uses, call in made(name, lambda x: x.requires_grad_()):
+            if name in uses:
+                with pytest.raises(RuntimeError, match="no backward"):
+                    call()
+                    pytest.fail(f"a gradient of {name} was lost")
+            with torch.no_grad():
+                call()
+    with torch.autograd.forward_ad.dual_level():
+        for _, call in made(None, None):
+            call()
+        for name in names:
+            for uses, call in made(name, lambda x: torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))):
+                if name in uses:
+                    with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode"):
+                        call()
+                        pytest.fail(f"a tangent of {name} was lost")
+    # transforms of torch.func hand in tensors without storage
+    pages, batch = pa.KVPages.create(1, 16, 2, 64, dtype=F32), pa.PagedBatch(_int([[0]] * n), _int([1] * n))
+    q = _randn(g, n, hq, d)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: pa.paged_attention(x, pages, batch), (q,), (q,))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: pa.paged_attention(x, pages, batch).sum())(q)
