@@ -1081,10 +1081,13 @@ static int check_attention(const lcmhip_kv_pages* pages, const lcmhip_paged_batc
 // and 387 / 292 us.
 // few: parts are added until the grid has kWantedFew workgroups, eight for each place on the chip, so that lists of unequal
 //      length even out (64 lists of 1000-3800 keys: 238 us with 2048 workgroups, 231 with 4096 or 8192).
+//      With a right max_q these are at most 16 kWantedFew partial (row, head) results; a max_q that understates the rows would have up
+//      to 64 for every row of the batch (16 GiB for 16384 rows of 32 heads of 128), so parts stop at kMaxPartials (0.5 GiB), which
+//      leaves batches with up to 16 times as many padding rows as they are.
 // many: a part takes a workgroup a step for each tile of keys and 3 us to begin and end, a round of kPlaces workgroups at a time,
 //      and its rows' partial results are written and read once (about 3 TB/s); the number of parts that makes the sum least.
 //      Twelve parts of a prefix of 3701 positions for 64 rows: 31.7 us, 4 parts 38.3, 32 parts 34.7.
-constexpr int kWantedFew = 4096, kPlaces = 512, kMaxParts = 64;
+constexpr int kWantedFew = 4096, kPlaces = 512, kMaxParts = 64, kMaxPartials = 1 << 20;
 struct ListPlan {
     bool many = false, alone = false;
     int tiles = 0;             // many: tiles of rows in all
@@ -1101,7 +1104,7 @@ static ListPlan plan_lists(int64_t lists, int64_t list_rows, int64_t all_rows, i
     p.many = list_rows > 16;
     if (!p.many) {
         const int64_t most = std::min<int64_t>(kMaxParts, (max_keys + kMinPartFew - 1) / kMinPartFew);
-        p.splits = (int)std::max<int64_t>(1, std::min(most, kWantedFew / std::max<int64_t>(lists * hk, 1)));
+        p.splits = (int)std::max<int64_t>(1, std::min({most, kWantedFew / (lists * hk), kMaxPartials / (all_rows * hk)}));
         // a wave for a part where four would have a group or two of keys each, once that still leaves every CU a workgroup
         p.alone = max_keys <= (int64_t)kMinPartFew * p.splits && lists * hk * p.splits >= 1024;
         return p;

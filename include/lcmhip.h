@@ -436,7 +436,7 @@ typedef struct {
     const int32_t* seq_lens;   /* (n_seqs) positions in the cache, the rows of this call included */
     const int32_t* q_starts;   /* (n_seqs + 1) or NULL: one row for every sequence */
     int32_t n_seqs, max_pages;
-    int32_t max_q;             /* the most rows of one sequence; chooses the kernel, a wrong value costs time only */
+    int32_t max_q;             /* the most rows of one sequence; chooses kernel and parts: a wrong value costs time and workspace, no result */
     int32_t max_keys;          /* upper bound of seq_lens, <= max_pages * page_size and <= 2^30 */
 } lcmhip_paged_batch;
 

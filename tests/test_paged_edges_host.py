@@ -1,0 +1,44 @@
+"""Edges of the paged cache entry points that need no GPU: workspaces, refusals, layouts."""
+
+import ctypes as C
+
+import pytest
+
+P = 4096                                 # a well-aligned address that nothing reads: no call here reaches a launch
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from lcm import _hip
+    return _hip
+
+
+def _pages(hip, **kw):
+    return hip.KVPages(**{**dict(k=P, v=P, n_pages=8, page_size=16, n_kv_heads=8, head_dim=128, dtype=1), **kw})
+
+
+def _batch(hip, **kw):
+    return hip.PagedBatch(**{**dict(page_table=P, seq_lens=P, q_starts=P, n_seqs=8, max_pages=1 << 16, max_q=1, max_keys=32768), **kw})
+
+
+def _workspace(hip, pages, batch, rows, heads, prefix=None):
+    n = C.c_size_t()
+    if prefix is None:
+        hip.check(hip.lib.lcmhip_paged_attention_workspace(pages, batch, rows, heads, C.byref(n)))
+    else:
+        hip.check(hip.lib.lcmhip_shared_prefix_attention_workspace(pages, batch, prefix, rows, heads, C.byref(n)))
+    return n.value
+
+
+def test_a_wrong_max_q_does_not_cost_gigabytes(hip):
+    """Partial results are (rows, heads) times the parts of a list; the number of parts is chosen for few rows a sequence, and a
+    max_q that understates them must not multiply it with all rows there are."""
+    partial = 4 * 128 + 8
+    for rows in (1 << 10, 1 << 14, 1 << 18, 1 << 22):
+        assert _workspace(hip, _pages(hip), _batch(hip), rows, 32) <= (1 << 20) * partial + 256
+        prefix = hip.SharedPrefix(page_table=P, lens=P, group_starts=P, n_groups=1 << 20, max_pages=1 << 16, max_keys=32768)
+        assert _workspace(hip, _pages(hip), _batch(hip), rows, 32, prefix) <= 2 * max(1 << 20, rows * 32) * partial + 256
+    # what a right max_q gives is as it was: 64 parts for two long sequences, padding rows among them, a few for many sequences
+    for rows in (2, 64, 512):
+        assert _workspace(hip, _pages(hip), _batch(hip, n_seqs=2, max_keys=131072), rows, 32) == 64 * rows * 32 * partial
+    assert _workspace(hip, _pages(hip, n_kv_heads=16), _batch(hip, n_seqs=64, max_keys=3800), 64, 16) == 4 * 64 * 16 * partial
