@@ -176,12 +176,17 @@ __global__ __launch_bounds__(256) void k_head_rows(HeadArgs a, int head_shift, i
                 for (int j = 0; j < 8; ++j) x[j] = __builtin_nanf("");
             }
         }
-        if (dst) store8<T>(dst, x);
+        store8<T>(dst, x);
     };
-    // heads [h, end) of one kind: from `src` (of head 0 of the kind, which is head `base` of the row) to `dst`
+    // heads [h, end) of one kind: from `src` (of head 0 of the kind, which is head `base` of the row) to `dst`; null, for a row that
+    // is skipped or whose page is not there: nothing is read
     auto heads = [&](int end, int base, const void* src, int64_t src_row, int64_t src_head, T* dst, int64_t dst_head, bool value,
                      const void* weight, const void* bias) {
         end = min(end, h1);
+        if (!dst) {                                        // the same for all lanes of a head
+            h += (max(end - h, 0) + hs - 1) >> head_shift << head_shift;
+            return;
+        }
         const T* from = reinterpret_cast<const T*>(src) + row * src_row + i0;
         float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
         if (weight) load8<T>(reinterpret_cast<const T*>(weight) + i0, w);
@@ -198,9 +203,9 @@ __global__ __launch_bounds__(256) void k_head_rows(HeadArgs a, int head_shift, i
                     h += it * hs;                          // the next kind begins here
                     return;
                 }
-                T* to = dst ? dst + (h + it * hs - base) * dst_head : nullptr;
+                T* to = dst + (h + it * hs - base) * dst_head;
                 if (!value) transform(raw[it], w, bias, to);
-                else if (to) *reinterpret_cast<Raw8<T>*>(to) = raw[it];
+                else *reinterpret_cast<Raw8<T>*>(to) = raw[it];
             }
         }
     };

@@ -183,3 +183,35 @@ def test_every_tensor_of_a_call_is_refused_with_a_gradient_or_a_tangent(pa):
         torch.func.jvp(lambda x: pa.paged_attention(x, pages, batch), (q,), (q,))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda x: pa.paged_attention(x, pages, batch).sum())(q)
+
+
+# ---- rows that are skipped -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_skipped_rows_between_others(pa, dtype):
+    """Rows of no sequence, of negative positions and of missing pages, alone in a wave or beside rows that are stored: what they
+    hold (NaN here) reaches nothing, their outputs stay, and their neighbours are as without them."""
+    g = _gen(23)
+    hq, hk, d, ps, rows = 5, 2, 64, 16, 77
+    x = _randn(g, rows, hq + 2 * hk, d, dtype=dtype)
+    starts, lens = [3, 20, 40, 70], [17, 30, 30]
+    table = _int([[0, 1], [2, -1], [3, 4]])
+    pos = _int([-1 if t % 3 == 0 else t for t in range(rows)])
+    seq = [next((b for b in range(3) if starts[b] <= t < starts[b + 1]), -1) for t in range(rows)]
+    at = [lens[seq[t]] - (starts[seq[t] + 1] - t) if seq[t] >= 0 else -1 for t in range(rows)]
+    lives = [t for t in range(rows) if seq[t] >= 0 and t % 3 and at[t] >= 0]
+    stored = [t for t in lives if int(table[seq[t], at[t] // ps]) >= 0]
+    rope, norm = pa.RotaryTable.create(128, d, style="halves"), pa.HeadNorm("rms", torch.ones(d, device="cuda", dtype=dtype), torch.ones(d, device="cuda", dtype=dtype))
+    x[[t for t in range(rows) if t not in lives]] = float("nan")
+    pages = pa.KVPages(torch.full((5, hk, ps, d), 5.0, device="cuda", dtype=dtype), torch.full((5, hk, ps, d), 6.0, device="cuda", dtype=dtype))
+    q_out = torch.full((rows, hq, d), 3.0, device="cuda", dtype=dtype)
+    pa.paged_append(pages, pa.PagedBatch(table, _int(lens), _int(starts), max_q=30), x[:, hq:hq + hk], x[:, hq + hk:], q=x[:, :hq], positions=pos,
+                    rope=rope, norm=norm, q_out=q_out)
+    alone_q, alone_k = pa.head_norm_rope(x[lives][:, :hq], x[lives][:, hq:hq + hk], positions=pos[lives].contiguous(), rope=rope, norm=norm)
+    want_q = torch.full_like(q_out, 3.0)
+    want_q[lives] = alone_q
+    assert torch.equal(q_out, want_q)
+    want_k, want_v = torch.full_like(pages.k, 5.0), torch.full_like(pages.v, 6.0)
+    for t in stored:
+        page, off = int(table[seq[t], at[t] // ps]), at[t] % ps
+        want_k[page, :, off], want_v[page, :, off] = alone_k[lives.index(t)], x[t, hq + hk:]
+    assert torch.equal(pages.k, want_k) and torch.equal(pages.v, want_v)
