@@ -150,14 +150,21 @@ struct Tile16<bf16_t, D> {
             for (int p = 0; p < 2; ++p) x[2 * h + p] = __builtin_amdgcn_perm(v[h][2 * p + 1][c / 2], v[h][2 * p][c / 2], sel);
         return __builtin_bit_cast(bf16x8_t, x);
     }
-    // Probabilities are rounded to bf16 for the second product (relative 2^-8 each, like the values they weigh); their sum
-    // is taken before, in fp32.
+    // A weight enters the second product as two bf16 numbers, its rounding and what that leaves (2^-16 of it is lost at most): the
+    // matrix unit has time for both while the wave waits for memory.
     __device__ __forceinline__ void weigh(const float (&p)[8], f32x4_t (&o)[kO]) const {
-        bf16x8_t pf;
+        bf16x8_t pf, rest;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pf[e] = (__bf16)p[e];
+        for (int e = 0; e < 8; ++e) {
+            pf[e] = (__bf16)p[e];
+            rest[e] = (__bf16)(p[e] - (float)pf[e]);
+        }
 #pragma unroll
-        for (int c = 0; c < kO; ++c) o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v_operand(c), pf, o[c], 0, 0, 0);
+        for (int c = 0; c < kO; ++c) {
+            const bf16x8_t x = v_operand(c);
+            o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, rest, o[c], 0, 0, 0);
+            o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pf, o[c], 0, 0, 0);
+        }
     }
     // The values of key i that are not finite alone, into the rows (lanes) that see it.
     __device__ __forceinline__ void weigh_not_finite(const float (&p)[8], f32x4_t (&o)[kO], int i, bool visible, int lane) const {
@@ -508,7 +515,9 @@ struct Tile32<bf16_t, D> {
         const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(base + (v_off[1] ^ (t << 6))));
         return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    // o += P V for a 32-key block; probabilities are rounded to bf16 as in Tile16
+    // o += P V for a 32-key block.  Weights are rounded to bf16 (2^-8 of each at most, like the values they weigh; their sum is taken
+    // before, in fp32): here the matrix unit is the bound, and the second product that Tile16 spends on what the rounding leaves takes
+    // 588 us instead of 446 on eight prompts of 1500-2048 rows, 236 instead of 207 on 192 rows over prefixes of 20k-32k positions.
     __device__ __forceinline__ static bf16x8_t p_operand(const f32x16_t& p, int u) {
         bf16x8_t pf;
 #pragma unroll

@@ -215,3 +215,42 @@ def test_skipped_rows_between_others(pa, dtype):
         page, off = int(table[seq[t], at[t] // ps]), at[t] % ps
         want_k[page, :, off], want_v[page, :, off] = alone_k[lives.index(t)], x[t, hq + hk:]
     assert torch.equal(pages.k, want_k) and torch.equal(pages.v, want_v)
+
+
+# ---- precision and long lists ----------------------------------------------------------------------------------------------------
+def _attend64(q, k, v, visible, scale, weight_error):
+    """q (n, hq, d), k / v (hk, keys, d) in 64 bits, visible (n, keys) (every row sees one): the result in 64 bits and its bound in
+    fp32 arithmetic whose weights are off by `weight_error` each."""
+    n, hq, d = q.shape
+    hk, keys, _ = k.shape
+    x = q.double().view(n, hk, hq // hk, d).permute(1, 2, 0, 3).reshape(hk, -1, d)
+    mask = visible[None, None].expand(hk, hq // hk, n, keys).reshape(hk, -1, keys)
+    s = (torch.bmm(x, k.transpose(1, 2).contiguous()) * scale).masked_fill(~mask, -torch.inf)
+    p = torch.softmax(s, -1)
+    out, spread = torch.bmm(p, v), torch.bmm(p, v.abs())
+    # a score: d products and sums, the scaling to base 2 and the subtraction of the maximum; exp2 itself 2 steps
+    size = torch.bmm(x.abs(), k.abs().transpose(1, 2).contiguous()).masked_fill(~mask, 0.0).amax(-1)
+    top = s.masked_fill(~mask, 0.0).abs().amax(-1)
+    ds = (d + 8) * ref.U32 * size * scale * 1.4427 + 4 * ref.U32 * top + 2 * ref.U32
+    many = (64 + mask.sum(-1) / 16 + 1) * ref.U32
+    bound = spread * (2 * ds + weight_error + 2 * many)[..., None]
+    back = lambda t: t.view(hk, hq // hk, n, d).permute(2, 0, 1, 3).reshape(n, hq, d)
+    return back(out), back(bound)
+
+
+@pytest.mark.parametrize("past,hq,hk,d,ps", [(137, 16, 16, 128, 16), (3000, 16, 4, 64, 64), (20000, 8, 8, 128, 128), (260, 5, 5, 64, 32)])
+def test_weights_of_few_rows_are_not_rounded_to_the_operand_type(pa, past, hq, hk, d, ps):
+    """With few rows a list the matrix unit waits for memory, and a weight enters the second product as two bf16 numbers: what is left
+    of it is off by half a step of a half step, 2^-16, and the output by its own rounding."""
+    g = _gen(past)
+    lens = [past, past // 2 + 1, 1]
+    each = -(-past // ps)
+    k, v = _randn(g, 3 * each, hk, ps, d, dtype=BF16, gain=1.5), _randn(g, 3 * each, hk, ps, d, dtype=BF16)
+    table = torch.randperm(3 * each, generator=g, device="cuda").to(torch.int32).view(3, each)
+    q = _randn(g, 3, hq, d, dtype=BF16, gain=0.5)
+    out = pa.paged_attention(q, pa.KVPages(k, v), pa.PagedBatch(table, _int(lens)))
+    for b in range(3):
+        kk, _ = ref.gather(k, table[b], lens[b], ps)
+        vv, _ = ref.gather(v, table[b], lens[b], ps)
+        want, bound = _attend64(q[b:b + 1], kk, vv, torch.ones(1, lens[b], dtype=torch.bool, device="cuda"), d ** -0.5, ref.half_step(BF16) ** 2)
+        _within(out[b:b + 1], want, ref.attend_bound(want, bound, BF16), b)
