@@ -150,20 +150,22 @@ struct Tile16<bf16_t, D> {
             for (int p = 0; p < 2; ++p) x[2 * h + p] = __builtin_amdgcn_perm(v[h][2 * p + 1][c / 2], v[h][2 * p][c / 2], sel);
         return __builtin_bit_cast(bf16x8_t, x);
     }
-    // A weight enters the second product as two bf16 numbers, its rounding and what that leaves (2^-16 of it is lost at most): the
-    // matrix unit has time for both while the wave waits for memory.
+    // A weight enters the second product as two bf16 numbers, its upper bits and the rest: the matrix unit has time for both while the
+    // wave waits for memory.  The upper bits are cut, not rounded, and the rest gets 2^-24 of the weight more: both are positive
+    // where the weight is, so that an infinite value stays one (a rest of 0, or below it, would make it NaN).  Cutting leaves a rest
+    // below 2^-7 of the weight, whose own rounding is 2^-8 of that: 2^-15 of the weight is lost at most.
     __device__ __forceinline__ void weigh(const float (&p)[8], f32x4_t (&o)[kO]) const {
-        bf16x8_t pf, rest;
+        u32x4_t cut;
+        bf16x8_t rest;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            pf[e] = (__bf16)p[e];
-            rest[e] = (__bf16)(p[e] - (float)pf[e]);
-        }
+        for (int e = 0; e < 8; ++e) rest[e] = (__bf16)fmaf(p[e], 0x1p-24f, p[e] - __uint_as_float(__float_as_uint(p[e]) & 0xffff0000u));
+#pragma unroll
+        for (int w = 0; w < 4; ++w) cut[w] = __builtin_amdgcn_perm(__float_as_uint(p[2 * w + 1]), __float_as_uint(p[2 * w]), 0x07060302u);
 #pragma unroll
         for (int c = 0; c < kO; ++c) {
             const bf16x8_t x = v_operand(c);
             o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, rest, o[c], 0, 0, 0);
-            o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pf, o[c], 0, 0, 0);
+            o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8_t, cut), o[c], 0, 0, 0);
         }
     }
     // The values of key i that are not finite alone, into the rows (lanes) that see it.

@@ -494,7 +494,7 @@ int lcmhip_paged_append(const lcmhip_kv_pages* pages, const lcmhip_paged_batch* 
  * (q_starts[b + 1] - t) + 1), otherwise all seq_lens[b]; of either those below max_keys.  A row that sees no key gives
  * zeros.  q (rows, n_heads, head_dim) strided, out the same contiguous; scale in [1e-20, 1e20].
  * Softmax statistics and sums are fp32.  Of bf16 operands, lists of keys with more than 16 (row, head) pairs a key head (prompts,
- * prefixes) have their weights rounded to bf16 for the product with the values; lists with fewer keep 16 bits of them.
+ * prefixes) have their weights rounded to bf16 for the product with the values; lists with fewer keep 15 bits of them.
  * `workspace` (device, 256-byte aligned) of at least lcmhip_paged_attention_workspace bytes holds partial results while the
  * call runs; nothing in it has to be zero and nothing is kept in it between calls, but calls that may overlap must not share
  * one.  bytes == 0: NULL will do. */

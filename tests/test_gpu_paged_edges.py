@@ -240,8 +240,9 @@ def _attend64(q, k, v, visible, scale, weight_error):
 
 @pytest.mark.parametrize("past,hq,hk,d,ps", [(137, 16, 16, 128, 16), (3000, 16, 4, 64, 64), (20000, 8, 8, 128, 128), (260, 5, 5, 64, 32)])
 def test_weights_of_few_rows_are_not_rounded_to_the_operand_type(pa, past, hq, hk, d, ps):
-    """With few rows a list the matrix unit waits for memory, and a weight enters the second product as two bf16 numbers: what is left
-    of it is off by half a step of a half step, 2^-16, and the output by its own rounding."""
+    """With few rows a list the matrix unit waits for memory, and a weight enters the second product as two bf16 numbers, its upper bits
+    and the rest.  Cutting a weight to bf16 leaves less than a step, finfo(bf16).eps = 2^-7 of it; the rest is rounded, half_step(bf16) =
+    2^-8 of itself: 2^-7 2^-8 = 2^-15 of the weight is lost at most, 2^-24 is added, and the output has its own rounding."""
     g = _gen(past)
     lens = [past, past // 2 + 1, 1]
     each = -(-past // ps)
@@ -252,5 +253,40 @@ def test_weights_of_few_rows_are_not_rounded_to_the_operand_type(pa, past, hq, h
     for b in range(3):
         kk, _ = ref.gather(k, table[b], lens[b], ps)
         vv, _ = ref.gather(v, table[b], lens[b], ps)
-        want, bound = _attend64(q[b:b + 1], kk, vv, torch.ones(1, lens[b], dtype=torch.bool, device="cuda"), d ** -0.5, ref.half_step(BF16) ** 2)
+        want, bound = _attend64(q[b:b + 1], kk, vv, torch.ones(1, lens[b], dtype=torch.bool, device="cuda"), d ** -0.5, 2.0 ** -15 + ref.U32)
         _within(out[b:b + 1], want, ref.attend_bound(want, bound, BF16), b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,past", [(1, 0), (1, 31), (1, 300), (3, 200), (40, 100)])
+def test_an_infinite_value_that_every_row_sees(pa, dtype, n, past):
+    """A value of +-inf under a weight that is not 0 gives +-inf in its dimension and nothing elsewhere, whatever the weight's low bits
+    are; both signs together give NaN."""
+    g = _gen(400 + n + past)
+    hq, hk, d, ps = 4, 2, 64, 16
+    each = -(-(past + n) // ps)
+    k, v = _randn(g, each, hk, ps, d, dtype=dtype), _randn(g, each, hk, ps, d, dtype=dtype)
+    table = torch.randperm(each, generator=g, device="cuda").to(torch.int32).view(1, each)
+    pages, batch = pa.KVPages(k, v), pa.PagedBatch(table, _int([past + n]), _int([0, n]), max_q=n)
+    q = _randn(g, n, hq, d, dtype=dtype, gain=0.5)
+    clean = pa.paged_attention(q, pages, batch)
+    for at in sorted({0, past // 3, past // 2, max(0, past - 1), past}):
+        page, off = int(table[0, at // ps]), at % ps
+        for head in range(hk):
+            kept = v[page, head, off].clone()
+            v[page, head, off, 7], v[page, head, off, 40] = float("inf"), -float("inf")
+            out = pa.paged_attention(q, pages, batch)
+            mine = torch.arange(hq, device="cuda") // (hq // hk) == head
+            assert torch.equal(out[:, ~mine], clean[:, ~mine])
+            hit, rest = out[:, mine], [x for x in range(d) if x not in (7, 40)]
+            assert (hit[..., 7] == float("inf")).all() and (hit[..., 40] == -float("inf")).all(), (at, head)
+            assert torch.equal(hit[..., rest], clean[:, mine][..., rest])
+            if past:                                               # another key's infinity of the other sign
+                other = (at + 1) % past if (at + 1) % past != at else 0
+                opage, ooff = int(table[0, other // ps]), other % ps
+                if (opage, ooff) != (page, off):
+                    okept = v[opage, head, ooff].clone()
+                    v[opage, head, ooff, 7] = -float("inf")
+                    assert torch.isnan(pa.paged_attention(q, pages, batch)[:, mine, 7]).all()
+                    v[opage, head, ooff] = okept
+            v[page, head, off] = kept
