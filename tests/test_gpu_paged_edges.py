@@ -290,3 +290,54 @@ def test_an_infinite_value_that_every_row_sees(pa, dtype, n, past):
                     assert torch.isnan(pa.paged_attention(q, pages, batch)[:, mine, 7]).all()
                     v[opage, head, ooff] = okept
             v[page, head, off] = kept
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("seqs,past,parts", [(32, (2000, 4000), 1), (16, (8000, 9000), 2)])
+def test_parts_of_more_pages_than_a_wave_holds(pa, dtype, causal, seqs, past, parts):
+    """Many rows against parts of more than 64 pages of 16: the page ids of a part are held 64 at a time.  Missing pages lie on both sides
+    of every 64th and on it; the pool is NaN wherever no sequence has a page."""
+    import ctypes as C
+    from lcm import _hip
+    g = _gen(seqs)
+    r = torch.Generator().manual_seed(seqs)
+    hq = hk = 8
+    d, ps = 64, 16
+    qs = [200 + int(torch.randint(0, 30, (1,), generator=r)) for _ in range(seqs)]
+    lens = [q + int(torch.randint(past[0], past[1] + 1, (1,), generator=r)) for q in qs]
+    counts = [-(-n // ps) for n in lens]
+    ids = torch.randperm(sum(counts) + 50, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((seqs, max(counts)), -1, dtype=torch.int32, device="cuda")
+    k = torch.full((sum(counts) + 50, hk, ps, d), float("nan"), dtype=dtype, device="cuda")
+    v = torch.full_like(k, float("nan"))
+    first = 0
+    for b, c in enumerate(counts):
+        mine = ids[first:first + c]
+        first += c
+        table[b, :c] = mine
+        k[mine.long()], v[mine.long()] = _randn(g, c, hk, ps, d, dtype=dtype, gain=1.5), _randn(g, c, hk, ps, d, dtype=dtype)
+    for b in range(seqs):                                              # a quarter of the sequences has all its pages
+        if b % 4:
+            for at in ([63, 64, 65, 128], [62, 127, 129], [64, 191, 192])[b % 4 - 1]:
+                if at < counts[b]:
+                    table[b, at] = (-1, k.shape[0], 2**31 - 1)[at % 3]
+    starts = [sum(qs[:i]) for i in range(seqs + 1)]
+    rows = starts[-1]
+    q = _randn(g, rows, hq, d, dtype=dtype, gain=1.0)
+    pages, batch = pa.KVPages(k, v), pa.PagedBatch(table, _int(lens), _int(starts), max_q=max(qs), max_keys=max(lens))
+    size = C.c_size_t()
+    _hip.check(_hip.lib.lcmhip_paged_attention_workspace(pages._ref, batch._bind(pages, rows), rows, hq, C.byref(size)))
+    assert size.value == (0 if parts == 1 else parts * rows * hq * (4 * d + 8))       # the parts are as long as this test wants them
+    out = pa.paged_attention(q, pages, batch, causal=causal)
+    for b in range(seqs):
+        kk, there = ref.gather(k, table[b], lens[b], ps)
+        vv, _ = ref.gather(v, table[b], lens[b], ps)
+        kk, vv = kk * 1, vv * 1
+        kk[:, ~there], vv[:, ~there] = 0.0, 0.0
+        visible = there[None].expand(qs[b], -1).clone()
+        if causal:
+            visible &= torch.arange(lens[b], device="cuda")[None] <= torch.arange(lens[b] - qs[b], lens[b], device="cuda")[:, None]
+        mine = slice(starts[b], starts[b + 1])
+        want, bound = _attend64(q[mine], kk, vv, visible, d ** -0.5, ref.half_step(dtype) if dtype is BF16 else 0.0)
+        _within(out[mine], want, ref.attend_bound(want, bound, dtype), b)
