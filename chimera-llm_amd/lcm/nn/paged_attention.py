@@ -30,6 +30,7 @@ from lcm.nn.normalization import norm_kind
 
 _lib = _hip.lib
 _NO_BACKWARD = "the paged cache operators have no backward: call them under torch.no_grad() or detach the inputs"
+_MOST = 2**30                             # of positions and rows: the structs hold 32-bit numbers, and ctypes cuts what does not fit
 _NO_TANGENT = "the paged cache operators have no forward-mode derivative: detach the inputs"
 
 
@@ -119,7 +120,7 @@ class PagedBatch:
     """The sequences of one step.  Sequence b owns the rows [q_starts[b], q_starts[b + 1]) of the q / k / v tensors (q_starts None:
     row b), its newest positions; seq_lens[b] counts its positions including them, and position c lies in page
     page_table[b, c // page_size].  `max_q` is the most rows of one sequence, `max_keys` an upper bound of seq_lens (None: what
-    the table can hold); both choose how the work is split.  Positions from max_keys on are not there: a row of such a position is
+    the table can hold, at most 2^30); both choose how the work is split.  Positions from max_keys on are not there: a row of such a position is
     not stored, and no row sees one."""
 
     def __init__(self, page_table: Tensor, seq_lens: Tensor, q_starts: Optional[Tensor] = None, max_q: int = 1,
@@ -136,7 +137,7 @@ class PagedBatch:
         _require(max_q >= 1, "max_q must be positive")
         _require(q_starts is not None or max_q == 1, "without q_starts every sequence has one row")
         self.page_table, self.seq_lens, self.q_starts = page_table, seq_lens, q_starts
-        self.num_seqs, self.max_pages, self.max_q, self.max_keys = n, page_table.shape[1], int(max_q), max_keys
+        self.num_seqs, self.max_pages, self.max_q, self.max_keys = n, page_table.shape[1], min(int(max_q), _MOST), max_keys
         self._fields, self._refs = (table, lens, starts, n, self.max_pages, self.max_q), {}
 
     def _bind(self, pages: KVPages, rows: int):
@@ -179,11 +180,11 @@ class SharedPrefix:
 
 
 def _reach(max_keys: Optional[int], max_pages: int, pages: KVPages) -> int:
-    reach = max_pages * pages.page_size
+    reach = min(max_pages * pages.page_size, _MOST)
     if max_keys is None:
-        return min(reach, 2**30)
+        return reach
     if not 1 <= max_keys <= reach:
-        raise ValueError(f"max_keys {max_keys} is not in [1, {reach}], what the page table holds")
+        raise ValueError(f"max_keys {max_keys} is not in [1, {reach}], what the page table holds and no more than 2^30")
     return max_keys
 
 

@@ -42,3 +42,14 @@ def test_a_wrong_max_q_does_not_cost_gigabytes(hip):
     for rows in (2, 64, 512):
         assert _workspace(hip, _pages(hip), _batch(hip, n_seqs=2, max_keys=131072), rows, 32) == 64 * rows * 32 * partial
     assert _workspace(hip, _pages(hip, n_kv_heads=16), _batch(hip, n_seqs=64, max_keys=3800), 64, 16) == 4 * 64 * 16 * partial
+
+
+def test_bounds_that_32_bits_would_cut_are_refused():
+    """The structs hold 32-bit numbers, and ctypes cuts what does not fit without a word: 2^32 + 16 would be 16."""
+    from types import SimpleNamespace
+    from lcm.nn import paged_attention as pa
+    wide = SimpleNamespace(page_size=65536)
+    for max_keys in (2**30 + 1, 2**31, 2**32 + 16):
+        with pytest.raises(ValueError, match="max_keys"):
+            pa._reach(max_keys, 1 << 20, wide)
+    assert pa._reach(2**30, 1 << 20, wide) == 2**30 and pa._reach(None, 1 << 20, wide) == 2**30 and pa._reach(None, 2, wide) == 131072
