@@ -64,7 +64,8 @@ class RotaryTable:
 
     @classmethod
     def create(cls, max_positions: int, rotary_dim: int, *, theta: float = 10000.0, style: str = "pairs", device=None) -> "RotaryTable":
-        """The table of angles p * theta^(-2 i / rotary_dim), computed in 64 bits."""
+        """The table of angles p * theta^(-2 i / rotary_dim), computed in 64 bits; rotary_dim a multiple of 16."""
+        _require(rotary_dim >= 16 and rotary_dim % 16 == 0, f"rotary_dim {rotary_dim} is not a positive multiple of 16")
         half = rotary_dim // 2
         freq = theta ** (-torch.arange(half, dtype=torch.float64) / half)
         angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * freq[None, :]

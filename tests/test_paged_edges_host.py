@@ -53,3 +53,11 @@ def test_bounds_that_32_bits_would_cut_are_refused():
         with pytest.raises(ValueError, match="max_keys"):
             pa._reach(max_keys, 1 << 20, wide)
     assert pa._reach(2**30, 1 << 20, wide) == 2**30 and pa._reach(None, 1 << 20, wide) == 2**30 and pa._reach(None, 2, wide) == 131072
+
+
+@pytest.mark.parametrize("rotary_dim", [33, 127, 1, 0, -16, 24])
+def test_a_rotary_table_of_an_odd_width_is_refused(rotary_dim):
+    """An odd width would lose a dimension and turn the others by angles of another width; only multiples of 16 can be used at all."""
+    from lcm.nn import paged_attention as pa
+    with pytest.raises(ValueError, match="rotary_dim"):
+        pa.RotaryTable.create(8, rotary_dim, device="cpu")
