@@ -79,6 +79,21 @@ inline int check_rows(const void* x, int64_t row, int64_t head, int dtype, const
     return LCMHIP_OK;
 }
 
+// Whether two of the pieces of `d` values at t row + h head, t < rows, h < heads, share a value.  Strides of either sign: turning an
+// axis round moves all pieces alike.
+inline bool rows_overlap(int64_t rows, int64_t heads, int64_t row_stride, int64_t head_stride, int64_t d) {
+    const __int128 row = row_stride < 0 ? -(__int128)row_stride : row_stride, head = head_stride < 0 ? -(__int128)head_stride : head_stride;
+    if (heads <= 1) return rows > 1 && row < d;
+    if (rows <= 1 || head < d) return head < d;
+    if (row >= (heads - 1) * head + d) return false;       // rows one behind the other, the ordinary case
+    if (row < d) return true;
+    for (int64_t h = 1; h < heads; ++h) {                  // the rows t that begin next before and behind head h of row 0
+        const __int128 t = h * head / row, before = h * head - t * row;
+        if ((t < rows && before < d) || (t + 1 < rows && row - before < d)) return true;
+    }
+    return false;
+}
+
 inline int page_shift_of(const lcmhip_kv_pages* p) { return __builtin_ctz((unsigned)p->page_size); }
 
 }  // namespace lcmhip

@@ -312,6 +312,8 @@ int lcmhip_head_norm_rope(const void* q, int64_t q_row, int64_t q_head, const vo
     LCM_TRY(check_rows(k_out, k_out_row, k_out_head, dtype, "head_norm_rope: k_out"));
     LCM_REQUIRE(q != q_out || !q || (q_row == q_out_row && q_head == q_out_head), "head_norm_rope: in place needs equal strides");
     LCM_REQUIRE(k != k_out || !k || (k_row == k_out_row && k_head == k_out_head), "head_norm_rope: in place needs equal strides");
+    LCM_REQUIRE(!q || !rows_overlap(rows, n_heads, q_out_row, q_out_head, head_dim), "head_norm_rope: rows of q_out lie on each other");
+    LCM_REQUIRE(!k || !rows_overlap(rows, n_kv_heads, k_out_row, k_out_head, head_dim), "head_norm_rope: rows of k_out lie on each other");
     HeadArgs a{};
     LCM_TRY(take_transform(a, norm, rotary, head_dim, q != nullptr, k != nullptr));
     a.q = q; a.q_row = q_row; a.q_head = q_head; a.k = k; a.k_row = k_row; a.k_head = k_head;

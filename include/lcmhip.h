@@ -474,7 +474,8 @@ typedef struct {
 /* Norm of every query and key head and the rotation behind it in one pass: y = rotate(norm(x)), fp32 inside, rounded once.
  * q, q_out (rows, n_heads, head_dim), k, k_out (rows, n_kv_heads, head_dim) with row / head strides; either pair may be NULL.
  * norm, rotary: NULL for none.  positions (rows) int32, required with rotary, else optional: rows of a negative position are
- * skipped (q_out, k_out keep what they hold), a position >= n_positions of a rotation gives NaN.  q_out may be q and k_out k (same strides). */
+ * skipped (q_out, k_out keep what they hold), a position >= n_positions of a rotation gives NaN.  q_out may be q and k_out k (same strides);
+ * outputs whose own rows or heads overlap are refused. */
 int lcmhip_head_norm_rope(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                           void* q_out, int64_t q_out_row, int64_t q_out_head, void* k_out, int64_t k_out_row, int64_t k_out_head,
                           int64_t rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const lcmhip_head_norm* norm,

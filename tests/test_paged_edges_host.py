@@ -61,3 +61,27 @@ def test_a_rotary_table_of_an_odd_width_is_refused(rotary_dim):
     from lcm.nn import paged_attention as pa
     with pytest.raises(ValueError, match="rotary_dim"):
         pa.RotaryTable.create(8, rotary_dim, device="cpu")
+
+
+def _overlap(rows, heads, d, row, head):
+    """Whether two (row, head) pieces of d values share one, by looking at all of them."""
+    starts = sorted(t * row + h * head for t in range(rows) for h in range(heads))
+    return any(b - a < d for a, b in zip(starts, starts[1:]))
+
+
+def test_outputs_whose_rows_lie_on_each_other_are_refused(hip):
+    """An expanded q_out, or one of overlapping rows, would be written by many waves at once.  Strides in units of 16 bytes."""
+    def call(rows, heads, row, head, which):
+        given, out, none = (P, heads * 128, 128), (P + (1 << 20), row, head), (None, 0, 0)
+        tensors = (*given, *none, *out, *none) if which == "q" else (*none, *given, *none, *out)
+        # a rotation of no positions ends every call that gets past the strides before it is launched
+        rot = hip.Rotary(cos=P, sin=P, n_positions=0, rotary_dim=64, style=0)
+        rc = hip.lib.lcmhip_head_norm_rope(*tensors, rows, heads, heads, 64, None, rot, P, 0, None)
+        assert rc == -1
+        return b"each other" in hip.lib.lcmhip_last_error()
+    for which in ("q", "k"):
+        for rows in (1, 2, 3, 7):
+            for heads in (1, 2, 5):
+                for row in (0, 32, 64, 128, 192, 256, 320, 448, 2240, -320):
+                    for head in (0, 64, 60, 96, 128, 192, 448, 704, -64):
+                        assert call(rows, heads, row, head, which) == _overlap(rows, heads, 64, row, head), (rows, heads, row, head)
