@@ -45,6 +45,7 @@ __device__ __forceinline__ int wave_count_le(const int32_t* ends, int n, int64_t
     return c;
 }
 
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;   // workgroups of 256: a launch holds fewer than 2^32 work items
 constexpr int kMaxKeys = 1 << 30;    // of one list: positions a few tiles behind the last are still int32
 
 inline int check_pages(const lcmhip_kv_pages* p) {

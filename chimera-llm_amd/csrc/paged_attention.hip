@@ -1162,13 +1162,16 @@ static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists&
         const int64_t parts = (int64_t)a.hk * ls.splits * (ls.many ? ls.tiles : ls.n);
         return ls.alone ? (parts + 3) / 4 : parts;
     };
-    const int64_t n1 = blocks_of(own);
-    LCM_REQUIRE(n1 <= INT32_MAX / 8, "paged attention: too many rows");
+    const int64_t n1 = blocks_of(own), n0 = prefix.n > 0 ? blocks_of(prefix) : 0, pair = (((n0 + 7) >> 3) + ((n1 + 7) >> 3)) << 3;
+    // joining: one group of lanes for a row while the rows alone fill the chip, else eight
+    const JoinArgs j{p.own.splits + p.prefix.splits, p.prefix.splits, prefix.group_starts, prefix.n};
+    const int64_t heads = (int64_t)a.rows * a.hq, per = 256 / (D / 4);
+    const bool wide = heads / per >= 256 || j.parts <= 8;
+    const int64_t n_join = wide ? (heads + per - 1) / per : (heads + per / 8 - 1) / (per / 8);
+    LCM_REQUIRE((prefix.n > 0 ? pair : n1) <= kMaxBlocks && (!p.joined || n_join <= kMaxBlocks),
+                "paged attention: too many rows or sequences, more workgroups than a launch holds");
     if (prefix.n > 0) {
-        const int64_t n0 = blocks_of(prefix);
-        LCM_REQUIRE(n0 <= INT32_MAX / 8, "paged attention: too many rows");
-        hipLaunchKernelGGL((k_paged_pair<T, D>), dim3((unsigned)((((n0 + 7) >> 3) + ((n1 + 7) >> 3)) << 3)), dim3(256), 0, st, a, prefix, own,
-                           (int)n0, (int)n1);
+        hipLaunchKernelGGL((k_paged_pair<T, D>), dim3((unsigned)pair), dim3(256), 0, st, a, prefix, own, (int)n0, (int)n1);
     } else if (own.many) {
         hipLaunchKernelGGL((k_paged_many<T, D>), dim3((unsigned)n1), dim3(256), 0, st, a, own);
     } else {
@@ -1176,13 +1179,8 @@ static int launch_paged(const PagedArgs& a, const KeyLists& own, const KeyLists&
     }
     LCM_HIP_CHECK(hipGetLastError());
     if (p.joined) {
-        // one group of lanes for a row while the rows alone fill the chip, else eight
-        const JoinArgs j{p.own.splits + p.prefix.splits, p.prefix.splits, prefix.group_starts, prefix.n};
-        const int64_t heads = (int64_t)a.rows * a.hq, per = 256 / (D / 4);
-        if (heads / per >= 256 || j.parts <= 8)
-            hipLaunchKernelGGL((k_paged_join<T, D, 1>), dim3((unsigned)((heads + per - 1) / per)), dim3(256), 0, st, a, j);
-        else
-            hipLaunchKernelGGL((k_paged_join<T, D, 8>), dim3((unsigned)((heads + per / 8 - 1) / (per / 8))), dim3(256), 0, st, a, j);
+        if (wide) hipLaunchKernelGGL((k_paged_join<T, D, 1>), dim3((unsigned)n_join), dim3(256), 0, st, a, j);
+        else hipLaunchKernelGGL((k_paged_join<T, D, 8>), dim3((unsigned)n_join), dim3(256), 0, st, a, j);
         LCM_HIP_CHECK(hipGetLastError());
     }
     return LCMHIP_OK;

@@ -242,7 +242,7 @@ static int launch_head_rows_t(const HeadArgs& a, hipStream_t st) {
     int64_t shares = std::min<int64_t>(turns, std::max<int64_t>(1, 1024 / blocks));
     const int each = (int)((turns + shares - 1) / shares);
     shares = (turns + each - 1) / each;
-    LCM_REQUIRE(blocks <= INT32_MAX && shares <= 65535, "head rows: too many rows or heads");
+    LCM_REQUIRE(blocks <= kMaxBlocks && shares <= 65535, "head rows: too many rows or heads, more workgroups than a launch holds");
     const dim3 grid((unsigned)blocks, (unsigned)shares);
     if (each > 1) hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 4>), grid, dim3(256), 0, st, a, shift, each << shift);
     else hipLaunchKernelGGL((k_head_rows<T, D, APPEND, 1>), grid, dim3(256), 0, st, a, shift, each << shift);

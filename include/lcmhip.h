@@ -416,6 +416,7 @@ int lcmhip_attention(const void* q, const void* k_cache, const void* v_cache, co
  *    (a sequence's rows keep their positions, counted back from its length); a negative length is 0; row ranges are cut to [0, rows];
  *  - rows that belong to no sequence (before q_starts[0], from q_starts[n_seqs] on), and rows that a call skips, are neither read nor
  *    written.
+ * A call that needs 2^24 workgroups or more in one launch (millions of sequences with many key heads) is refused.
  * Row pointers are 16-byte aligned and their strides (in elements) a multiple of 16 bytes; the last dimension is dense.
  * head_dim is 64 or 128, page_size a power of two from 16 to 65536, n_heads a multiple of n_kv_heads (query head h reads key head
  * h / (n_heads / n_kv_heads)).  Outputs must not overlap inputs unless a comment says so. */

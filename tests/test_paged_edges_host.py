@@ -85,3 +85,23 @@ def test_outputs_whose_rows_lie_on_each_other_are_refused(hip):
                 for row in (0, 32, 64, 128, 192, 256, 320, 448, 2240, -320):
                     for head in (0, 64, 60, 96, 128, 192, 448, 704, -64):
                         assert call(rows, heads, row, head, which) == _overlap(rows, heads, 64, row, head), (rows, heads, row, head)
+
+
+def test_grids_past_the_launch_limit_are_refused(hip):
+    """A launch holds fewer than 2^32 work items a dimension, 2^24 workgroups of 256: what needs more is refused by name and before
+    anything is launched, not by the runtime behind the first kernel."""
+    def refused(rc, text=b"workgroups"):
+        return rc == -1 and text in hip.lib.lcmhip_last_error()
+    one = dict(max_pages=1, max_keys=16)
+    many_seqs = _batch(hip, n_seqs=1 << 21, q_starts=None)
+    assert refused(hip.lib.lcmhip_paged_attention(_pages(hip), many_seqs, P, 1024, 128, P, 1 << 21, 8, 0.1, 1, P, 1 << 40, None))
+    # the few-row kernel of one prefix's rows and the joining kernel behind it: rows of 128 heads, 2^27 results
+    prefix = hip.SharedPrefix(page_table=P, lens=P, group_starts=P, n_groups=1 << 20, max_pages=1, max_keys=16)
+    rows = (1 << 20) + 8
+    wide = _pages(hip, n_kv_heads=1)
+    assert refused(hip.lib.lcmhip_shared_prefix_attention(wide, _batch(hip, n_seqs=rows, q_starts=None, **one), prefix, P, 16384, 128, P, rows, 128, 0.1, 1,
+                                                          P, 1 << 60, None))
+    # heads: eight rows of eight heads a workgroup at head_dim 64, so 2^30 rows are 2^28 workgroups
+    assert refused(hip.lib.lcmhip_head_norm_rope(P, 512, 64, None, 0, 0, P + (1 << 20), 512, 64, None, 0, 0, 1 << 30, 8, 0, 64, None, None, None, 1, None))
+    assert refused(hip.lib.lcmhip_paged_append(_pages(hip), _batch(hip, **one), P, 1024, 128, P, 1024, 128, None, 0, 0, None, 1 << 28, 0,
+                                               None, None, None, None))
