@@ -283,8 +283,9 @@ struct Tile16<float, D> {
 // Bound by the bytes of the keys and values: with one row a list 15 of the 16 columns of a product are empty, and the matrix unit
 // is still busy for less than a third of the time the bytes take.  Two rounds of loads are in flight for every wave (the values of
 // this group, the keys of the next), 128 KB a CU.  One row for each of 64 documents of 1000-3800 keys, 16 heads, bf16: 208 us, 6.3
-// TB/s; two sequences of 120k-131k keys, 8 key heads: 154 us and 5 for the join, 6.2 TB/s; one of 137 keys, fp32: 9 us, of which
-// the chain length -> page -> keys -> values -> join is all.  Eight waves instead of four made that one slower (9.2 against 7.7 us
+// TB/s; two sequences of 120k-131k keys, 8 key heads: 155 us and 5 for the join, 6.2 TB/s; one of 137 keys, fp32: 9.4 us a call, all
+// of it the chain length -> page -> keys -> values -> join.  Each of its three rounds waits for its own keys: the next page id is
+// looked up inside the loop and one group of keys is in flight.  Eight waves instead of four made that one slower (9.2 against 7.7 us
 // launch to launch).
 template <int D>
 struct FewShared {
@@ -726,7 +727,7 @@ __device__ __forceinline__ void lds_dma(const char* base, const uint32_t (&off)[
 // LDS-DMA brings one tile ahead.  Two workgroups a CU.
 // Bound by the matrix instructions at the clock that the chip's power leaves them: a stream of them from registers on random data
 // reaches 1500-1700 TFLOP/s in bf16, a large library product 1380, this kernel 1080 on 16384 rows that see 16384 keys, 1020 causal,
-// 900 on eight causal prompts of 1500-2048 rows behind up to 2048 cached positions (450 us), where beginning and ending a
+// 900 on eight causal prompts of 1500-2048 rows behind up to 2048 cached positions (438-451 us), where beginning and ending a
 // workgroup and the tiles on the diagonal count.  Without the LDS-DMA that took 418 of then 470 us, without the exponentials as
 // well 393, with nothing but the products 320.  Measured and left: eight waves that share 256 rows, with two to four buffers (465
 // against 456 us, short prompts 139 against 112), the loop unrolled twice, operands read six or eight products ahead.
@@ -1124,7 +1125,9 @@ static ListPlan plan_lists(int64_t lists, int64_t list_rows, int64_t all_rows, i
     // workgroups of one part, if the lists have about as many rows each
     const int64_t blocks = hk * std::max((all_rows + 127) / 128, lists * ((all_rows / lists + 127) / 128));
     const int step_keys = dtype == LCMHIP_BF16 ? 64 : 32;
-    const double step_us = (dtype == LCMHIP_BF16 ? 0.9 : 6.8) * head_dim / 128;   // two workgroups a CU at the matrix unit's rate
+    // Two workgroups a CU at the matrix unit's nominal rate.  512 workgroups do 2.15 GFLOP in a bf16 step, which the kernel does in
+    // 2.0-2.4 us when the chip is full: joins and the fixed 3 us weigh about twice too much in large bf16 calls.
+    const double step_us = (dtype == LCMHIP_BF16 ? 0.9 : 6.8) * head_dim / 128;
     const double join_us = (double)all_rows * hk * head_dim * 8 / 3e6;
     const int most = std::min(kMaxParts, (max_keys + 2 * step_keys - 1) / (2 * step_keys));
     double best = 0;

@@ -8,9 +8,10 @@
 // in fp32, rounded once when it is stored.  The sums run over the D / 8 lanes of a head; the partner of a pair (i, i + 1) is
 // in the same lane, that of (i, i + rotary_dim / 2) rotary_dim / 16 lanes away.
 //
-// Bound by bytes read and written, each once: 16384 rows of 32 + 8 heads of 128, bf16, in 65 us (5.3 TB/s; a large copy reaches 5.0),
-// 13 thousand rows of 32 + 8 + 8 heads appended behind ragged histories in 65 us (5.1 TB/s); 64 rows in 3.6 us, a launch.  A head at
-// a time, with its angles and its place looked up for each, took 96 and 127 us: 220 vector operations a kilobyte.
+// Bound by bytes read and written, each once: 16384 rows of 32 + 8 heads of 128, bf16, in 64 us a call and 59 in the kernel (5.8 TB/s; a
+// large copy reaches 5.0), 13 thousand rows of 32 + 8 + 8 heads appended behind ragged histories in 65 and 56 us (5.9 TB/s); 64 rows in
+// 3.6 us, a launch.  A head at a time, with its angles and its place looked up for each, took 96 and 127 us a call: 220 vector
+// operations a kilobyte.
 #include <algorithm>
 
 #include "paged.h"
@@ -34,7 +35,8 @@ struct HeadArgs {
     int n_seqs, max_keys;
 };
 
-// Eight values as they lie in memory, read past the caches: nobody reads them again (append of 13 thousand rows: 67 -> 60 us).
+// Eight values as they lie in memory, read past the caches: nobody reads them again (append of 13 thousand rows, calls: 67 -> 60 us on
+// one card).
 // What is written stays in reach of the attention behind.
 template <typename T>
 struct Raw8;

@@ -417,6 +417,10 @@ int lcmhip_attention(const void* q, const void* k_cache, const void* v_cache, co
  *  - rows that belong to no sequence (before q_starts[0], from q_starts[n_seqs] on), and rows that a call skips, are neither read nor
  *    written.
  * A call that needs 2^24 workgroups or more in one launch (millions of sequences with many key heads) is refused.
+ * A key or value that is NaN or infinite reaches the rows that see it and no others.  An infinite value gives an infinity, or NaN
+ * where infinities of both signs are seen or its weight leaves fp32 on the way (how far below the largest score that is depends on
+ * the order of the keys).  Values are summed with their weights, at most 2^8 each, in fp32 before the division: |value| times the
+ * number of keys has to stay below 2^120.
  * Row pointers are 16-byte aligned and their strides (in elements) a multiple of 16 bytes; the last dimension is dense.
  * head_dim is 64 or 128, page_size a power of two from 16 to 65536, n_heads a multiple of n_kv_heads (query head h reads key head
  * h / (n_heads / n_kv_heads)).  Outputs must not overlap inputs unless a comment says so. */
